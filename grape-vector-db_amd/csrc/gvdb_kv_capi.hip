@@ -1,0 +1,267 @@
+// gvdb_kv_capi.hip — C ABI of the token cache (include/gvdb.h, gvdb_kv_*):
+// checks of arguments, the split of the work, the scratch layout.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "gvdb_internal.h"
+#include "gvdb_kv.h"
+
+using namespace gvdb;
+
+namespace {
+
+gvdb_status invalid(const char* msg) { return report_status(GVDB_ERR_INVALID_ARGUMENT, msg); }
+
+// Entered with the cache's device current, left with the caller's.
+struct DeviceScope {
+    int before = -1;
+    hipError_t err;
+    explicit DeviceScope(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) {
+            err = hipSetDevice(device);
+        } else {
+            before = -1;
+        }
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// No C++ exception crosses the boundary.
+template <class F>
+gvdb_status guarded(F&& f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        return GVDB_ERR_OUT_OF_MEMORY;
+    }
+}
+
+gvdb_status launch(int device, const char* what, hipError_t (*run)(const void*, hipStream_t), const void* args, void* stream) {
+    DeviceScope scope(device);
+    hipError_t e = scope.err;
+    if (e == hipSuccess) e = run(args, (hipStream_t)stream);
+    if (e == hipSuccess) return GVDB_OK;
+    return report_status(e == hipErrorOutOfMemory ? GVDB_ERR_OUT_OF_MEMORY : GVDB_ERR_DEVICE,
+                         std::string(what) + ": " + hipGetErrorString(e));
+}
+
+uint32_t size_of(uint32_t dtype) { return dtype == GVDB_F32 ? 4 : 2; }
+
+gvdb_status take_cache(const gvdb_kv_cache* in, KvCache& c) {
+    if (!in) return invalid("token cache: null cache");
+    if (in->head_dim != 64 && in->head_dim != 128 && in->head_dim != 256)
+        return report_status(GVDB_ERR_INVALID_VECTOR_DIMENSION, "token cache: head_dim is 64, 128 or 256");
+    if (in->page_size == 0 || in->page_size % 32 || in->page_size > 1024)
+        return invalid("token cache: page_size is a multiple of 32, at most 1024");
+    if (in->kv_heads == 0 || in->kv_heads > 4096) return invalid("token cache: kv_heads is 1 .. 4096");
+    if (in->n_pages == 0 || in->n_pages > (1ull << 31)) return invalid("token cache: n_pages is 1 .. 2^31");
+    if (in->device < 0) return invalid("token cache: negative device");
+    if (!in->pool || !in->bounds || !in->bound_exps) return invalid("token cache: null buffer");
+    if (((uintptr_t)in->pool | (uintptr_t)in->bounds) & 15u) return invalid("token cache: pool and bounds are 16-byte aligned");
+    c = {in->pool, in->bounds, in->bound_exps, in->n_pages, in->kv_heads, in->head_dim, in->page_size};
+    return GVDB_OK;
+}
+
+gvdb_status take_batch(const gvdb_kv_batch* in, const KvCache& c, KvBatch& bt) {
+    if (!in) return invalid("token cache: null batch");
+    if (in->rows > 0x7FFFFFFFu) return invalid("token cache: over 2^31 - 1 rows");
+    if (in->rows == 0) {
+        bt = {};
+        return GVDB_OK;
+    }
+    if (in->n_seqs == 0 || in->n_seqs > 0x7FFFFFFFu) return invalid("token cache: rows without a sequence");
+    if (!in->page_table || !in->lengths) return invalid("token cache: null page_table or lengths");
+    if (in->table_width == 0 || in->table_width > 0x7FFFFFFFu / c.page) return invalid("token cache: table_width * page_size is 1 .. 2^31 - 1");
+    if (in->n_seqs > 1 && in->table_stride < in->table_width) return invalid("token cache: table_stride below table_width");
+    if (!in->cu && in->rows % in->n_seqs) return invalid("token cache: without cu, rows is a multiple of n_seqs");
+    bt = {in->page_table, in->table_stride, in->table_width, in->n_seqs, in->lengths, in->cu, in->rows, in->max_new, in->max_len};
+    // hints: never over what the sizes allow
+    if (!bt.cu) bt.max_new = bt.rows / bt.n_seqs;
+    if (bt.max_new == 0 || bt.max_new > bt.rows) bt.max_new = bt.rows;
+    const uint64_t most = (uint64_t)bt.table_width * c.page;
+    if (bt.max_len == 0 || bt.max_len > most) bt.max_len = (uint32_t)most;
+    return GVDB_OK;
+}
+
+gvdb_status take_rows(const gvdb_kv_rows* in, const char* what, KvRows& r) {
+    if (!in || !in->data) return invalid((std::string("token cache: null ") + what).c_str());
+    if (in->dtype > GVDB_BF16) return invalid((std::string("token cache: unknown dtype of ") + what).c_str());
+    const uint32_t size = size_of(in->dtype);
+    if ((uintptr_t)in->data % size) return invalid((std::string("token cache: misaligned ") + what).c_str());
+    r = {in->data, in->dtype, in->row_stride, in->head_stride, false};
+    r.wide = ((uint64_t)(uintptr_t)in->data | (uint64_t)in->row_stride * size | (uint64_t)in->head_stride * size) % 16 == 0;
+    return GVDB_OK;
+}
+
+uint64_t up256(uint64_t n) { return (n + 255) / 256 * 256; }
+
+// How the work is cut, and where in the scratch each part lies.
+struct Plan {
+    AttendArgs a{};
+    uint64_t scores = 0, chosen = 0, part_o = 0, part_ml = 0, bytes = 0;
+};
+
+gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t q_heads, uint32_t top, Plan& p) {
+    if (q_heads == 0 || q_heads % c.heads || q_heads > 65536)
+        return invalid("token cache: q_heads is a multiple of kv_heads, at most 65536");
+    if (top > 65536) return invalid("token cache: top is at most 65536");
+    const uint64_t group = q_heads / c.heads;
+    AttendArgs& a = p.a;
+    a.q_heads = q_heads;
+    a.top = top;
+    const uint64_t tiles = top ? (uint64_t)std::min(top, bt.table_width) * (c.page / 32) : ((uint64_t)bt.max_len + 31) / 32;
+    const uint64_t rows_each = top ? group : bt.max_new * group;
+    const uint64_t units0 = top ? bt.rows : bt.n_seqs;
+    uint64_t row_tiles = (rows_each + 15) / 16;
+    // grids stay below 2^20 tiles of rows where the hints are loose: the kernels stride over the rest
+    row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
+    const uint64_t units = units0 * c.heads * row_tiles;
+    // keys are split until about 1024 workgroups have work, in parts of at least 8 tiles
+    const uint64_t chunk = std::max<uint64_t>(8, (units * tiles + 1023) / 1024);
+    uint64_t splits = std::max<uint64_t>(1, (tiles + chunk - 1) / chunk);
+    a.row_tiles = (uint32_t)row_tiles;
+    a.splits = (uint32_t)splits;
+    a.chunk = (uint32_t)chunk;
+    if (units * splits > 0x7FFFFFFFull) return invalid("token cache: too many rows and heads for one call");
+    const uint64_t qr = (uint64_t)bt.rows * q_heads;
+    uint64_t at = 0;
+    if (top) {
+        a.score_chunk = 256;
+        p.scores = at;
+        at += up256((uint64_t)bt.rows * c.heads * bt.table_width * 4);
+        p.chosen = at;
+        at += up256((uint64_t)bt.rows * c.heads * top * 4);
+    }
+    if (splits > 1) {
+        p.part_o = at;
+        at += up256(qr * splits * c.dim * 4);
+        p.part_ml = at;
+        at += up256(qr * splits * 8);
+    }
+    p.bytes = at;
+    return GVDB_OK;
+}
+
+struct KvCall {
+    KvCache c;
+    KvBatch bt;
+    KvRows k, v;
+    AttendArgs a;
+};
+
+gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q, uint32_t q_heads, float scale,
+                   int32_t causal, uint32_t top, uint32_t first, uint32_t recent, const gvdb_kv_rows* out, int32_t* chosen,
+                   float* lse, void* scratch, uint64_t scratch_bytes, bool choose, void* stream) {
+    KvCall call{};
+    if (gvdb_status s = take_cache(cache, call.c)) return s;
+    if (gvdb_status s = take_batch(batch, call.c, call.bt)) return s;
+    if (choose && top == 0) return invalid("token cache: top is at least 1");
+    if (choose && (uint64_t)first + recent > top) return invalid("token cache: first + recent is at most top");
+    if (!std::isfinite(scale)) return invalid("token cache: scale is not finite");
+    if (call.bt.rows == 0) return GVDB_OK;
+    Plan p;
+    if (gvdb_status s = plan_attend(call.c, call.bt, q_heads, choose ? top : 0, p)) return s;
+    if (gvdb_status s = take_rows(q, "q", p.a.q)) return s;
+    if (gvdb_status s = take_rows(out, "out", p.a.out)) return s;
+    if (p.a.q.dtype != p.a.out.dtype) return invalid("token cache: q and out are of one dtype");
+    if (p.bytes && !scratch) return invalid("token cache: null scratch");
+    if (scratch_bytes < p.bytes) return invalid("token cache: scratch below gvdb_kv_scratch_bytes");
+    if ((uintptr_t)scratch & 15u) return invalid("token cache: scratch is 16-byte aligned");
+    AttendArgs& a = p.a;
+    uint8_t* base = (uint8_t*)scratch;
+    a.lse = lse;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.causal = causal != 0;
+    a.first = first;
+    a.recent = recent;
+    a.part_o = (float*)(base + p.part_o);
+    a.part_ml = (float*)(base + p.part_ml);
+    a.scores = (float*)(base + p.scores);
+    a.chosen = chosen ? chosen : (int32_t*)(base + p.chosen);
+    call.a = a;
+    if (choose)
+        return launch(cache->device, "kv_attend_topk",
+                      [](const void* x, hipStream_t s) { auto& k = *(const KvCall*)x; return launch_kv_attend_topk(k.c, k.bt, k.a, s); },
+                      &call, stream);
+    return launch(cache->device, "kv_attend",
+                  [](const void* x, hipStream_t s) { auto& k = *(const KvCall*)x; return launch_kv_attend(k.c, k.bt, k.a, s); }, &call,
+                  stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+gvdb_status gvdb_kv_append_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
+                                  const gvdb_kv_rows* v, void* stream) {
+    return guarded([&]() -> gvdb_status {
+        KvCall call{};
+        if (gvdb_status s = take_cache(cache, call.c)) return s;
+        if (gvdb_status s = take_batch(batch, call.c, call.bt)) return s;
+        if (call.bt.rows == 0) return GVDB_OK;
+        if (gvdb_status s = take_rows(k, "k", call.k)) return s;
+        if (gvdb_status s = take_rows(v, "v", call.v)) return s;
+        if (call.k.dtype != call.v.dtype) return invalid("token cache: k and v are of one dtype");
+        return launch(cache->device, "kv_append",
+                      [](const void* x, hipStream_t s) { auto& a = *(const KvCall*)x; return launch_kv_append(a.c, a.bt, a.k, a.v, s); },
+                      &call, stream);
+    });
+}
+
+gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
+                                const gvdb_kv_rows* v, void* stream) {
+    return guarded([&]() -> gvdb_status {
+        KvCall call{};
+        if (gvdb_status s = take_cache(cache, call.c)) return s;
+        if (gvdb_status s = take_batch(batch, call.c, call.bt)) return s;
+        if (call.bt.rows == 0 || (!k && !v)) return GVDB_OK;
+        if (k)
+            if (gvdb_status s = take_rows(k, "k", call.k)) return s;
+        if (v)
+            if (gvdb_status s = take_rows(v, "v", call.v)) return s;
+        if (k && v && call.k.dtype != call.v.dtype) return invalid("token cache: k and v are of one dtype");
+        return launch(cache->device, "kv_read",
+                      [](const void* x, hipStream_t s) { auto& a = *(const KvCall*)x; return launch_kv_read(a.c, a.bt, a.k, a.v, s); },
+                      &call, stream);
+    });
+}
+
+gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t q_heads, uint32_t top,
+                                  uint64_t* bytes) {
+    return guarded([&]() -> gvdb_status {
+        if (!bytes) return invalid("token cache: null bytes");
+        *bytes = 0;
+        KvCache c{};
+        KvBatch bt{};
+        if (gvdb_status s = take_cache(cache, c)) return s;
+        if (gvdb_status s = take_batch(batch, c, bt)) return s;
+        if (bt.rows == 0) return GVDB_OK;
+        Plan p;
+        if (gvdb_status s = plan_attend(c, bt, q_heads, top, p)) return s;
+        *bytes = p.bytes;
+        return GVDB_OK;
+    });
+}
+
+gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q, uint32_t q_heads,
+                                  float scale, int32_t causal, const gvdb_kv_rows* out, float* lse, void* scratch,
+                                  uint64_t scratch_bytes, void* stream) {
+    return guarded([&] {
+        return attend(cache, batch, q, q_heads, scale, causal, 0, 0, 0, out, nullptr, lse, scratch, scratch_bytes, false, stream);
+    });
+}
+
+gvdb_status gvdb_kv_attend_topk_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
+                                       uint32_t q_heads, float scale, uint32_t top, uint32_t first, uint32_t recent,
+                                       const gvdb_kv_rows* out, int32_t* chosen, float* lse, void* scratch, uint64_t scratch_bytes,
+                                       void* stream) {
+    return guarded([&] {
+        return attend(cache, batch, q, q_heads, scale, 1, top, first, recent, out, chosen, lse, scratch, scratch_bytes, true, stream);
+    });
+}
+
+}  // extern "C"

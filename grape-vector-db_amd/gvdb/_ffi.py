@@ -31,6 +31,7 @@ GVDB_METRIC_L2 = 1
 GVDB_METRIC_COSINE_DISTANCE = 2
 GVDB_SEARCH_BQ_RERANK = 0
 GVDB_SEARCH_FLAT = 1
+GVDB_F32, GVDB_F16, GVDB_BF16 = 0, 1, 2
 GVDB_N_POISONED = 0xFFFFFFFF
 GVDB_COMM_ID_BYTES = 128
 
@@ -88,6 +89,44 @@ class gvdb_persist_meta(C.Structure):
         ("ef_search", C.c_uint64),
         ("max_layers", C.c_uint64),
         ("created_at", C.c_char * 64),
+    ]
+
+
+class gvdb_kv_cache(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("bounds", C.c_void_p),
+        ("bound_exps", C.c_void_p),
+        ("n_pages", C.c_uint64),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("device", C.c_int32),
+    ]
+
+
+class gvdb_kv_batch(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p),
+        ("table_stride", C.c_uint64),
+        ("table_width", C.c_uint32),
+        ("n_seqs", C.c_uint32),
+        ("lengths", C.c_void_p),
+        ("cu", C.c_void_p),
+        ("rows", C.c_uint32),
+        ("max_new", C.c_uint32),
+        ("max_len", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class gvdb_kv_rows(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("row_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("dtype", C.c_uint32),
+        ("reserved", C.c_uint32),
     ]
 
 
@@ -171,6 +210,11 @@ SIGNATURES = {
     "gvdb_sparse_search_bm25": (C.c_int, [P, P, P, P, u64, u64, P, P, P]),
     "gvdb_rrf_fuse": (C.c_int, [P, P, P, u32, P, P, P, u32, P, P, P, u32, u64, f32, u64, P, P, P, P]),
     "gvdb_rrf_fuse_device": (C.c_int, [P, P, P, u32, P, P, P, u32, P, P, P, u32, u64, f32, u64, P, P, P, P, P]),
+    "gvdb_kv_append_device": (C.c_int, [P, P, P, P, P]),
+    "gvdb_kv_read_device": (C.c_int, [P, P, P, P, P]),
+    "gvdb_kv_scratch_bytes": (C.c_int, [P, P, u32, u32, PU64]),
+    "gvdb_kv_attend_device": (C.c_int, [P, P, P, u32, f32, i32, P, P, P, u64, P]),
+    "gvdb_kv_attend_topk_device": (C.c_int, [P, P, P, u32, f32, u32, u32, u32, P, P, P, P, u64, P]),
 }
 
 _lib = None

@@ -512,6 +512,115 @@ gvdb_status gvdb_rrf_fuse_device(const uint64_t* d_dense_ids, const float* d_den
                                  float k, uint64_t limit, uint64_t* d_out_ids, float* d_out_scores,
                                  float* d_out_breakdown, uint32_t* d_out_n, void* stream);
 
+/* ---- token cache: a model's keys and values, paged, in 4 bits --------------
+ * A store of key and value vectors that a language model reads by inner
+ * product at every token, beside the index that retrieves what it reads.  It
+ * keeps the index's scheme: vectors are quantised as they are written
+ * (gvdb_bq_quantize), a cheap score over small codes selects, and what was
+ * selected is scored exactly (the two stages of gvdb_index_search).
+ *
+ * The caller owns the cache's three device buffers (16-byte aligned, any
+ * contents to begin with) and hands out its pages; nothing is kept between
+ * calls.  Per page of page_size tokens and key/value head:
+ *   pool        page_size / 32 tiles of 34 * head_dim bytes: key codes (16 D),
+ *               key scales (D), value codes (16 D), value scales (D) of 32 tokens
+ *   bounds      int8 [2][head_dim]: the largest and the smallest stored key per
+ *               channel, rounded outward, in units of 2^(bound_exps - 133)
+ *   bound_exps  uint8: 255 = a key of the page is not finite
+ * A code is a sign and one of {0, .5, 1, 1.5, 2, 3, 4, 6} (nearest, ties to
+ * the even code) times 2^(scale - 127); 32 neighbouring channels share a scale:
+ * the smallest with max|x| < 7 * 2^(scale - 127), within 2 .. 252.  Scale 255:
+ * the group held an infinity or a NaN and reads as NaN.  Scales are
+ * [D / 32][32 tokens] bytes.  Byte b of token t's D / 2 code bytes (channels 2b
+ * and 2b + 1, the even one in the low half) lies at
+ *   keys:   u = (t % 2) * (D / 8) + b % (D / 8),
+ *           ((u / 16) * 64 + b / (D / 8) * 16 + t / 2) * 16 + u % 16
+ *   values: u = (t % 8) * (D / 32) + b % (D / 32),
+ *           ((u / 16) * 64 + t / 8 * 16 + b / (D / 32)) * 16 + u % 16
+ *
+ * All calls enqueue on `stream` and return without waiting; they allocate
+ * nothing and may be captured into a graph.  Argument errors are returned
+ * before anything is enqueued.  What only the device knows is checked there: a
+ * page number outside [0, n_pages) or beyond table_width is never followed
+ * (append skips its tokens, read and attention give NaN for what needs it). */
+typedef enum gvdb_dtype { GVDB_F32 = 0, GVDB_F16 = 1, GVDB_BF16 = 2 } gvdb_dtype;
+
+typedef struct gvdb_kv_cache {
+    uint8_t* pool;            /* [n_pages][kv_heads][page_size / 32][34 * head_dim] */
+    int8_t* bounds;           /* [n_pages][kv_heads][2][head_dim] */
+    uint8_t* bound_exps;      /* [n_pages][kv_heads] */
+    uint64_t n_pages;
+    uint32_t kv_heads;
+    uint32_t head_dim;        /* 64, 128 or 256 */
+    uint32_t page_size;       /* tokens: a multiple of 32, at most 1024 */
+    int32_t device;           /* HIP device ordinal of the buffers and of the call */
+} gvdb_kv_cache;
+
+/* The sequences of a call.  Sequence s owns rows cu[s] .. cu[s + 1] of the row
+ * tensors (k, v, q, out); cu == NULL: rows / n_seqs each.  Rows behind the last
+ * sequence belong to none and are left as they were.  A length below 0 is 0. */
+typedef struct gvdb_kv_batch {
+    const int32_t* page_table; /* device [n_seqs][table_stride]: pages in token order */
+    uint64_t table_stride;     /* entries between sequences */
+    uint32_t table_width;      /* pages that a sequence may use */
+    uint32_t n_seqs;
+    const int32_t* lengths;    /* device [n_seqs]: append, read: tokens before the call's first;
+                                * attention: tokens in the cache, the call's own among them */
+    const int32_t* cu;         /* device [n_seqs + 1], not decreasing, or NULL */
+    uint32_t rows;             /* rows of the tensors, at most 2^31 - 1 */
+    uint32_t max_new;          /* most rows of one sequence, 0 = not known; sizes the grid only */
+    uint32_t max_len;          /* largest length, 0 = not known; sizes the grid only */
+    uint32_t reserved;
+} gvdb_kv_batch;
+
+/* [rows][heads][head_dim] on the device, neighbouring channels side by side. */
+typedef struct gvdb_kv_rows {
+    void* data;
+    int64_t row_stride;        /* elements */
+    int64_t head_stride;
+    uint32_t dtype;            /* gvdb_dtype */
+    uint32_t reserved;
+} gvdb_kv_rows;
+
+/* Quantises rows k and v into tokens lengths[s] .. of each sequence and makes
+ * the touched pages' bounds new over every token that they hold up to there.
+ * Tokens behind stay what they were.  A page must not be written for two
+ * sequences in one call. */
+gvdb_status gvdb_kv_append_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
+                                  const gvdb_kv_rows* v, void* stream);
+/* The stored values of the same tokens, rounded once to the rows' type.
+ * k or v may be NULL. */
+gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
+                                const gvdb_kv_rows* v, void* stream);
+/* Scratch of the attention calls (top: 0 for gvdb_kv_attend_device). */
+gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t q_heads,
+                                  uint32_t top, uint64_t* bytes);
+/* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the tokens that
+ * row r sees: with `causal`, row i of a sequence's n sees the first
+ * length - n + i + 1 of its length tokens, else all of them.  Query head h
+ * reads key/value head h / (q_heads / kv_heads).  A row that sees no token is 0
+ * (lse: -inf).  lse: device [rows][q_heads] f32, the natural logarithm of the
+ * softmax's denominator, or NULL.  q and out: one type, q_heads heads.  Sums and
+ * statistics are kept in 32 bits; keys, values and queries enter the products
+ * exactly, the probabilities in 8 bits for bf16 rows, 16 for f16, 24 for f32. */
+gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
+                                  uint32_t q_heads, float scale, int32_t causal, const gvdb_kv_rows* out, float* lse,
+                                  void* scratch, uint64_t scratch_bytes, void* stream);
+/* The same over `top` pages that each row and key/value head takes of those it
+ * sees: the first `first`, the last `recent` (its own is the last), then those
+ * of the largest score, the lowest page among equals.  score(page) = the
+ * largest over the group's query heads of
+ *   sum_d max(q8_d, 0) hi_d + min(q8_d, 0) lo_d,  q8 = rint(q / 2^a),
+ * an upper estimate of the page's largest q . k (2^a: the smallest under which
+ * |q8| <= 127); the sum runs over whole numbers and is exact.  A page whose
+ * bounds are not finite comes first.  chosen: device int32
+ * [rows][kv_heads][top], ascending positions in the page table, -1 behind the
+ * last, or NULL. */
+gvdb_status gvdb_kv_attend_topk_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
+                                       uint32_t q_heads, float scale, uint32_t top, uint32_t first, uint32_t recent,
+                                       const gvdb_kv_rows* out, int32_t* chosen, float* lse, void* scratch,
+                                       uint64_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,508 @@
+"""GPU: the token cache's operators against their definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import kv_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+HALF = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}   # a rounding is off by at most this, relatively
+TINY = {"bf16": 2.0 ** -133, "f16": 2.0 ** -25, "f32": 2.0 ** -149}  # ... or this, below the normal range
+PROB = {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}   # the probabilities' bits
+
+
+@pytest.fixture()
+def kv(gvdb_mod):
+    from gvdb import kv
+
+    return kv
+
+
+class Store:
+    """A cache filled through append, and the stored values in 64 bits.  Whatever was not written reads as NaN."""
+
+    def __init__(self, kv, seed, dtype, heads, D, page, lens, spread=1.0, width=None):
+        rng = np.random.default_rng(seed)
+        need = [-(-n // page) for n in lens]
+        self.width = width or max(1, max(need)) + 1
+        self.n_pages = sum(need) + 2
+        order = rng.permutation(self.n_pages)
+        table = np.full((len(lens), self.width), -7, np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            table[s, :n] = order[at:at + n]
+            at += n
+        self.cache = kv.KvCache(self.n_pages, heads, D, page)
+        self.cache.pool.fill_(255)
+        self.cache.bounds.fill_(-1)
+        self.cache.bound_exps.fill_(255)
+        self.table = torch.from_numpy(table).cuda()
+        self.lens, self.page, self.heads, self.D, self.dtype = list(lens), page, heads, D, dtype
+        self.k, self.v = [], []
+        rows_k, rows_v = [], []
+        for n in lens:
+            k = rng.standard_normal((n, heads, D)) + rng.standard_normal((1, heads, D))
+            k[:, :, : D // 16] *= 4
+            k += 0.7 * np.repeat(rng.standard_normal((n // 16 + 1, heads, D)), 16, 0)[:n]
+            rows_k.append(torch.from_numpy(k * spread).to(DT[dtype]))
+            rows_v.append(torch.from_numpy(rng.standard_normal((n, heads, D))).to(DT[dtype]))
+        self.cu = torch.from_numpy(np.cumsum([0] + list(lens)).astype(np.int32)).cuda()
+        k, v = torch.cat(rows_k), torch.cat(rows_v)
+        if len(k):
+            self.cache.append(k.cuda(), v.cuda(), self.table, self.zeros(), cu=self.cu)
+        for a, b in zip(rows_k, rows_v):
+            self.k.append(plain.stored(a.double().numpy()))
+            self.v.append(plain.stored(b.double().numpy()))
+
+    def zeros(self):
+        return torch.zeros(len(self.lens), dtype=torch.int32, device="cuda")
+
+    def lengths(self):
+        return torch.tensor(self.lens, dtype=torch.int32, device="cuda")
+
+    def bounds(self, s, h):
+        n, P = self.lens[s], self.page
+        return [plain.bounds(self.k[s][p:min(p + P, n), h]) for p in range(0, n, P)]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def queries(seed, dtype, new, heads, D):
+    rng = np.random.default_rng(seed)
+    return torch.from_numpy(rng.standard_normal((sum(new), heads, D))).to(DT[dtype])
+
+
+def check_attend(st, q, new, out, lse=None, causal=True, scale=None, chosen=None, skip=()):
+    """Every output within its bound: the output's rounding, the probabilities' bits, and 32-bit sums of scores and products."""
+    D, dtype = st.D, st.dtype
+    scale = D ** -0.5 if scale is None else scale
+    Hq = q.shape[1]
+    g = Hq // st.heads
+    out = out.double().cpu().numpy()
+    qd = q.double().cpu().numpy()
+    row = 0
+    for s, n in enumerate(new):
+        L = st.lens[s]
+        for i in range(n):
+            for hq in range(Hq):
+                if (row, hq) in skip:
+                    continue
+                h = hq // g
+                sees = np.arange(L) < (L - n + i + 1 if causal else L)
+                if chosen is not None:
+                    mine = np.isin(np.arange(L) // st.page, chosen[row, h][chosen[row, h] >= 0])
+                    sees &= mine
+                o, ls, absum, s1 = plain.attend(qd[row, hq], st.k[s][:, h], st.v[s][:, h], scale, sees)
+                # a score is off by (D + 8) roundings of its terms' sum, a sum of n terms by n / 32 + 64 roundings
+                rel = 2 * (D + 8) * 2.0 ** -24 * s1 + (L / 32 + 64) * 2.0 ** -23
+                tol = HALF[dtype] * np.abs(o) + (PROB[dtype] + rel) * (1 + HALF[dtype]) * absum + TINY[dtype]
+                err = np.abs(out[row, hq] - o)
+                assert (err <= tol).all(), (s, i, hq, float((err / np.maximum(tol, 1e-300)).max()))
+                if lse is not None:
+                    got = float(lse[row, hq])
+                    assert got == ls if np.isinf(ls) else abs(got - ls) <= rel + 2.0 ** -22 * (abs(ls) + 8), (s, i, hq, got, ls)
+            row += 1
+
+
+# ---- append and read ----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,heads,D,page,lens", [
+    ("bf16", 2, 128, 64, (1, 63, 64, 65, 200)),
+    ("f32", 3, 64, 32, (31, 0, 97, 1)),
+    ("f16", 1, 256, 128, (130, 5)),
+    ("f32", 2, 128, 96, (300,)),
+])
+def test_append_stores_what_it_should(kv, dtype, heads, D, page, lens):
+    st = Store(kv, 1, dtype, heads, D, page, lens)
+    k, v = st.cache.read(st.table, st.zeros(), sum(lens), cu=st.cu, dtype=torch.float32)
+    k, v = k.double().cpu().numpy(), v.double().cpu().numpy()
+    assert np.array_equal(k, np.concatenate(st.k)) and np.array_equal(v, np.concatenate(st.v))
+    # the buffers are laid out as documented
+    pool, b8, be = st.cache.pool.cpu().numpy(), st.cache.bounds.cpu().numpy(), st.cache.bound_exps.cpu().numpy()
+    table = st.table.cpu().numpy()
+    used = set()
+    for s, n in enumerate(lens):
+        for h in range(heads):
+            for j, want in enumerate(st.bounds(s, h)):
+                pg = table[s, j]
+                used.add(int(pg))
+                assert np.array_equal(b8[pg, h], want[0]) and be[pg, h] == want[1]
+                for t in range(0, min(page, n - j * page), 32):
+                    a, b = plain.tile_values(pool[pg, h, t // 32], D)
+                    m = min(32, n - j * page - t)
+                    assert np.array_equal(a[:m], st.k[s][j * page + t:j * page + t + m, h])
+                    assert np.array_equal(b[:m], st.v[s][j * page + t:j * page + t + m, h])
+                    # what lies behind was left alone
+                    assert np.isnan(a[m:]).all() and np.isnan(b[m:]).all()
+    for pg in set(range(st.n_pages)) - used:
+        assert (pool[pg] == 255).all() and (be[pg] == 255).all() and (b8[pg] == -1).all()
+
+
+def test_append_in_pieces_is_append_at_once(kv):
+    """Token by token, in runs over page borders, and written twice: the same bytes."""
+    D, heads, page, n = 128, 2, 64, 200
+    x = torch.randn(n, heads, D, dtype=torch.bfloat16, device="cuda")
+    y = torch.randn(n, heads, D, dtype=torch.bfloat16, device="cuda")
+    table = i32([[3, 0, 4, 2]])
+    got = []
+    for cuts in ([0, n], list(range(n + 1)), [0, 1, 63, 64, 130, n], [0, 150, n]):
+        c = kv.KvCache(5, heads, D, page)
+        c.pool.zero_(), c.bounds.zero_(), c.bound_exps.zero_()
+        for a, b in zip(cuts, cuts[1:]):
+            c.append(x[a:b], y[a:b], table, i32([a]))
+        c.append(x[17:90], y[17:90], table, i32([17]), max_new=1) if cuts[1] == 150 else None
+        if cuts[1] == 150:  # the rewrite ended inside a page: its bounds cover what it wrote up to there
+            c.append(x[64:128], y[64:128], table, i32([64]))
+        got.append((c.pool.clone(), c.bounds.clone(), c.bound_exps.clone()))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+
+
+def test_append_extremes(kv):
+    """Zeros, the smallest and largest floats, ties, infinities and NaN."""
+    D = 64
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((40, 1, D)).astype(np.float32)
+    x[0] = 0
+    x[1] = 1e-45
+    x[2] *= 1e-38
+    x[3] = 3.4028235e38
+    x[4] *= 1e37
+    x[5, 0, :32] = np.array([6, 5, 3.5, 2.5, 1.75, 1.25, .75, .25] * 4) * np.tile([1, -1], 16)
+    x[6, 0, 32:] = np.array([7, 5, 3.5, 2.5, 1.75, 1.25, .75, .25] * 4)
+    x[7, 0, 3] = np.inf
+    x[8, 0, 40] = -np.inf
+    x[9, 0, 10] = np.nan
+    x[10, 0, 0] = np.float32(6.9999995)
+    want = plain.stored(x.astype(np.float64))
+    c = kv.KvCache(2, 1, D, 32)
+    t = torch.from_numpy(x).cuda()
+    c.append(t, t.flip(2), i32([[1, 0]]), i32([0]))
+    k, v = c.read(i32([[1, 0]]), i32([0]), 40, dtype=torch.float32)
+    assert np.array_equal(k.double().cpu().numpy(), want, equal_nan=True)
+    assert np.array_equal(v.flip(2).double().cpu().numpy()[10:], want[10:], equal_nan=True)
+    assert c.bound_exps.cpu().tolist()[1] == [255] and c.bound_exps.cpu().tolist()[0] != [255]
+
+
+def test_append_and_read_strided_and_misaligned(kv):
+    D, heads = 128, 3
+    base = torch.randn(50, 2 * heads + 1, D, device="cuda").to(torch.float16)
+    k, v = base[:, :heads], base[:, heads:2 * heads]
+    off = torch.randn(50 * heads * D + 3, device="cuda").to(torch.float16)[3:].view(50, heads, D)
+    table = i32([[0, 1]])
+    for a, b in ((k, v), (off, v), (k.flip(0).transpose(0, 1).contiguous().transpose(0, 1), off)):
+        c = kv.KvCache(2, heads, D, 32)
+        c.append(a, b, table, i32([0]))
+        out = torch.full((2, 50, heads, 2 * D), 7.0, dtype=torch.float16, device="cuda")
+        c.read(table, i32([0]), 50, out=(out[0, :, :, :D], out[1, :, :, 1:D + 1]))
+        assert np.array_equal(out[0, :, :, :D].double().cpu().numpy(), plain.stored(a.double().cpu().numpy()))
+        assert np.array_equal(out[1, :, :, 1:D + 1].double().cpu().numpy(), plain.stored(b.double().cpu().numpy()))
+        assert (out[0, :, :, D:] == 7).all() and (out[1, :, :, 0] == 7).all() and (out[1, :, :, D + 1:] == 7).all()
+
+
+def test_pages_that_are_not_there(kv):
+    """No page number is followed out of the pool or the table: append skips, read and attention give NaN."""
+    D, page = 64, 32
+    x = torch.randn(3 * 96, 1, D, device="cuda")
+    table = i32([[0, -1, 1], [2, 3, 99], [4, 5, 6]])
+    c = kv.KvCache(7, 1, D, page)
+    c.append(x, x, table, i32([0, 0, 0]))
+    k, v = c.read(table, i32([0, 0, 0]), 288, dtype=torch.float32)
+    k = k.view(3, 96, D)
+    want = plain.stored(x.double().cpu().numpy()).reshape(3, 96, D)
+    bad = np.zeros((3, 96), bool)
+    bad[0, 32:64] = bad[1, 64:] = True
+    assert torch.isnan(k).all(-1).squeeze().cpu().numpy().reshape(3, 96).tolist() == bad.tolist()
+    assert np.array_equal(k.double().cpu().numpy()[~bad], want[~bad])
+    q = torch.randn(6, 2, D, device="cuda")
+    for lens, nan in (((33, 64, 96), (0,)), ((32, 65, 96), (1,)), ((32, 64, 97), (2,))):
+        for o in (c.attend(q, table, i32(lens)), c.attend_topk(q, table, i32(lens), 3)[0]):
+            got = torch.isnan(o).flatten(1).all(1).cpu().view(3, 2)[:, 1].nonzero().flatten().tolist()
+            assert got == list(nan), (lens, got)
+            fine = torch.isfinite(o).flatten(1).all(1).cpu().view(3, 2)
+            assert all(fine[s, 1] for s in range(3) if s not in nan)
+
+
+# ---- attention ------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,Hq,heads,D,page,lens,new", [
+    ("bf16", 8, 2, 128, 64, (1,), (1,)),
+    ("bf16", 32, 8, 128, 64, (777, 0, 1, 64, 65, 1500), (1,) * 6),
+    ("f16", 6, 2, 64, 32, (300, 33, 31), (1, 1, 1)),
+    ("f32", 4, 4, 256, 128, (129, 500), (1, 1)),
+    ("f32", 7, 1, 128, 32, (250,), (1,)),
+    ("bf16", 40, 2, 64, 32, (100, 999), (1, 1)),          # more heads a group than a tile has rows
+    ("f16", 4, 2, 128, 64, (40, 3, 130), (5, 5, 5)),      # a sequence shorter than its rows: the first see nothing
+    ("bf16", 8, 2, 128, 64, (65, 300), (65, 37)),
+    ("f32", 3, 1, 64, 96, (100, 0, 50), (100, 4, 50)),
+    ("f16", 5, 5, 256, 32, (70, 41), (33, 41)),
+    ("bf16", 12, 4, 64, 64, (260,), (131,)),
+])
+def test_attend(kv, dtype, Hq, heads, D, page, lens, new):
+    st = Store(kv, 2, dtype, heads, D, page, lens)
+    q = queries(3, dtype, new, Hq, D).cuda()
+    cu = i32(np.cumsum((0,) + new).tolist())
+    lse = torch.full(q.shape[:2], 5.0, device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), cu=cu, lse=lse, max_new=max(new), max_len=max(lens))
+    check_attend(st, q, new, out, lse)
+    if len(set(new)) == 1:
+        assert torch.equal(out, st.cache.attend(q, st.table, st.lengths(), max_len=max(lens)))
+    # hints size the launch only: too small, too large and none give the same sums up to their order
+    for hints in ({"max_new": 1, "max_len": 1}, {}, {"max_new": 10 ** 6, "max_len": 10 ** 6}):
+        check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), cu=cu, **hints))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attend_without_causal_and_with_scale(kv, dtype):
+    st = Store(kv, 4, dtype, 2, 128, 64, (90, 10, 0))
+    new = (4, 20, 3)
+    q = queries(5, dtype, new, 4, 128).cuda()
+    cu = i32([0, 4, 24, 27])
+    lse = torch.empty(27, 4, device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), cu=cu, causal=False, scale=-0.3, lse=lse)
+    check_attend(st, q, new, out, lse, causal=False, scale=-0.3)
+
+
+@pytest.mark.parametrize("dtype,lens", [("bf16", (9000, 4001)), ("f16", (20000,)), ("f32", (6001, 5, 7777))])
+def test_attend_split_along_the_keys(kv, dtype, lens):
+    """Few rows and long contexts: the parts are joined by a second kernel, alike on every run."""
+    st = Store(kv, 6, dtype, 2, 128, 64, lens)
+    q = queries(7, dtype, (1,) * len(lens), 6, 128).cuda()
+    lse = torch.empty(len(lens), 6, device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), lse=lse)
+    check_attend(st, q, (1,) * len(lens), out, lse)
+    for _ in range(3):
+        assert torch.equal(out, st.cache.attend(q, st.table, st.lengths()))
+
+
+@pytest.mark.parametrize("dtype,spread", [("bf16", 30.0), ("f32", 30.0), ("f16", 1e-3)])
+def test_attend_sharp_and_flat(kv, dtype, spread):
+    st = Store(kv, 8, dtype, 1, 64, 32, (500,), spread)
+    q = queries(9, dtype, (3,), 4, 64).cuda()
+    check_attend(st, q, (3,), st.cache.attend(q, st.table, st.lengths()))
+
+
+def test_what_is_masked_may_hold_anything(kv):
+    """A key or value that is not finite shows in the rows that see it, and in no other; a value only in its group of channels."""
+    D, page = 128, 64
+    for poison in (float("nan"), float("inf"), -float("inf")):
+        st = Store(kv, 10, "f32", 1, D, page, (150,))
+        k = torch.from_numpy(np.random.default_rng(1).standard_normal((4, 1, D))).float().cuda()
+        v = k.clone()
+        v[1, 0, 40] = poison   # token 121: a value, channels 32 .. 63
+        k[3, 0, 7] = poison    # token 123: a key
+        st.cache.append(k, v, st.table, i32([120]))
+        st.k[0][120:124], st.v[0][120:124] = plain.stored(k.double().cpu().numpy()), plain.stored(v.double().cpu().numpy())
+        q = queries(11, "f32", (150,), 2, D).cuda()
+        lse = torch.empty(150, 2, device="cuda")
+        out = st.cache.attend(q, st.table, st.lengths(), lse=lse)
+        nan = torch.isnan(out).cpu().numpy()
+        want = np.zeros((150, 2, D), bool)
+        want[121:, :, 32:64] = True
+        want[123:] = True
+        assert np.array_equal(nan, want)
+        skip = {(r, h) for r in range(121, 150) for h in range(2)}
+        check_attend(st, q, (150,), out, skip=skip)
+        # single tokens over a shorter length
+        for n, bad in ((121, False), (122, True), (124, True)):
+            one = st.cache.attend(q[:1], st.table, i32([n]))
+            assert bool(torch.isnan(one).any()) == bad
+            assert bool(torch.isnan(one).all()) == (n == 124)
+    # a query that is not finite spoils its own row alone
+    st = Store(kv, 12, "bf16", 2, 64, 32, (80, 80))
+    q = queries(13, "bf16", (2, 2), 4, 64).cuda()
+    q[1, 2, 5] = float("nan")
+    out = st.cache.attend(q, st.table, st.lengths())
+    assert torch.isnan(out[1, 2]).all()
+    check_attend(st, q, (2, 2), out, skip={(1, 2)})
+
+
+def test_strided_misaligned_and_given_outputs(kv):
+    D, Hq, heads = 128, 4, 2
+    st = Store(kv, 14, "bf16", heads, D, 64, (100, 70))
+    fused = torch.randn(10, Hq + 2 * heads, D, device="cuda").to(torch.bfloat16)
+    new = (4, 3)
+    cu = i32([0, 4, 7])  # rows 7 .. 9 belong to no sequence
+    flat = torch.randn(10 * Hq * D + 1, device="cuda").to(torch.bfloat16)[1:].view(10, Hq, D)
+    for q in (fused[:, :Hq], flat):
+        big = torch.full((10, Hq, D + 5), 3.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((10, Hq), 3.0, device="cuda")
+        out = st.cache.attend(q, st.table, st.lengths(), cu=cu, out=big[:, :, 2:D + 2], lse=lse)
+        check_attend(st, q, new, out, lse)
+        assert (big[7:] == 3).all() and (big[:, :, :2] == 3).all() and (big[:, :, D + 2:] == 3).all() and (lse[7:] == 3).all()
+        got, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 4, cu=cu)
+        check_attend(st, q, new, got, chosen=chosen.cpu().numpy())
+        assert (got[7:] == 0).all() and (chosen[7:] == -1).all()
+
+
+# ---- attention over chosen pages --------------------------------------------------------------
+@pytest.mark.parametrize("dtype,Hq,heads,D,page,lens,new,top,first,recent", [
+    ("bf16", 8, 2, 128, 64, (5000,), (1,), 8, 1, 1),
+    ("bf16", 32, 8, 128, 64, (3000, 0, 1, 64, 65, 2111), (1,) * 6, 6, 1, 2),
+    ("f16", 6, 2, 64, 32, (900, 40), (3, 2), 5, 0, 0),
+    ("f32", 5, 5, 256, 32, (700, 310), (1, 4), 4, 2, 2),
+    ("f32", 20, 1, 64, 32, (600,), (2,), 7, 1, 1),
+    ("bf16", 3, 1, 128, 128, (2000, 7, 30), (9, 7, 40), 3, 1, 1),
+    ("f16", 4, 4, 128, 32, (500,), (40,), 100, 1, 1),     # more than there are: everything
+    ("bf16", 4, 2, 64, 32, (300, 200), (1, 1), 1, 0, 1),
+])
+def test_attend_topk(kv, dtype, Hq, heads, D, page, lens, new, top, first, recent):
+    st = Store(kv, 15, dtype, heads, D, page, lens)
+    q = queries(16, dtype, new, Hq, D).cuda()
+    cu = i32(np.cumsum((0,) + new).tolist())
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), top, first=first, recent=recent, cu=cu, lse=lse, max_new=max(new),
+                                       max_len=max(lens))
+    got = chosen.cpu().numpy()
+    qd = q.double().cpu().numpy()
+    g = Hq // heads
+    row = 0
+    for s, n in enumerate(new):
+        bounds = [st.bounds(s, h) for h in range(heads)]
+        for i in range(n):
+            place = lens[s] - n + i
+            seen = place // page + 1 if place >= 0 else 0
+            for h in range(heads):
+                want = plain.choose(qd[row, h * g:(h + 1) * g], bounds[h], seen, top, first, recent)
+                assert got[row, h].tolist() == want + [-1] * (top - len(want)), (s, i, h)
+            row += 1
+    check_attend(st, q, new, out, lse, chosen=got)
+    for hints in ({"max_new": 1, "max_len": 1}, {}):
+        o2, c2 = st.cache.attend_topk(q, st.table, st.lengths(), top, first=first, recent=recent, cu=cu, **hints)
+        assert torch.equal(c2, chosen)
+        check_attend(st, q, new, o2, chosen=got)
+
+
+def test_topk_ties_take_the_lowest_page(kv):
+    """Equal pages score alike: the lowest of them are taken; all-zero queries and keys too."""
+    D, page = 64, 32
+    c = kv.KvCache(40, 1, D, page)
+    x = torch.randn(page, 1, D, device="cuda").repeat(40, 1, 1)
+    table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(1, 2, D, device="cuda")
+    for k, qq in ((x, q), (x, q * 0), (x * 0, q)):
+        c.append(k, k, table, i32([0]))
+        _, chosen = c.attend_topk(qq, table, i32([40 * page]), 5, first=0, recent=1)
+        assert chosen.flatten().tolist() == [0, 1, 2, 3, 39]
+
+
+def test_topk_takes_pages_that_are_not_finite(kv):
+    st = Store(kv, 17, "f32", 1, 64, 32, (640,))
+    k = torch.randn(1, 1, 64, device="cuda")
+    k[0, 0, 3] = float("nan")
+    st.cache.append(k, k, st.table, i32([32 * 11 + 31]))
+    q = queries(18, "f32", (1,), 2, 64).cuda()
+    out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 4)
+    assert 11 in chosen.flatten().tolist() and torch.isnan(out).all()
+
+
+def test_topk_of_everything_is_attend(kv):
+    st = Store(kv, 19, "bf16", 2, 128, 64, (1000, 77))
+    q = queries(20, "bf16", (3, 3), 8, 128).cuda()
+    out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 16)
+    check_attend(st, q, (3, 3), out)
+    check_attend(st, q, (3, 3), st.cache.attend(q, st.table, st.lengths()))
+
+
+# ---- together ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,page,dtype", [(128, 64, "bf16"), (64, 32, "f16")])
+def test_serving_run(kv, D, page, dtype):
+    """Prompts, then tokens one by one: append, attend over everything, attend over chosen pages, at every step."""
+    Hq, heads, lens, steps = 8, 2, [90, 1, 200], 40
+    st = Store(kv, 21, dtype, heads, D, page, lens, width=8)
+    free = iter(range(st.n_pages, st.n_pages + 20))
+    big = kv.KvCache(st.n_pages + 20, heads, D, page)
+    big.pool.fill_(255)
+    big.pool[:st.n_pages], big.bounds[:st.n_pages], big.bound_exps[:st.n_pages] = st.cache.pool, st.cache.bounds, st.cache.bound_exps
+    st.cache = big
+    rng = np.random.default_rng(22)
+    for _ in range(steps):
+        for s, n in enumerate(st.lens):
+            if n % page == 0:
+                st.table[s, n // page] = next(free)
+        k, v = (torch.from_numpy(rng.standard_normal((3, heads, D))).to(DT[dtype]) for _ in range(2))
+        q = torch.from_numpy(rng.standard_normal((3, Hq, D))).to(DT[dtype]).cuda()
+        st.cache.append(k.cuda(), v.cuda(), st.table, st.lengths())
+        for s in range(3):
+            st.k[s] = np.concatenate([st.k[s], plain.stored(k[s:s + 1].double().numpy())])
+            st.v[s] = np.concatenate([st.v[s], plain.stored(v[s:s + 1].double().numpy())])
+            st.lens[s] += 1
+        check_attend(st, q, (1, 1, 1), st.cache.attend(q, st.table, st.lengths()))
+        out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 2)
+        check_attend(st, q, (1, 1, 1), out, chosen=chosen.cpu().numpy())
+
+
+def test_another_stream(kv):
+    st = Store(kv, 23, "bf16", 2, 128, 64, (3000, 500))
+    q = queries(24, "bf16", (1, 1), 8, 128).cuda()
+    want = st.cache.attend(q, st.table, st.lengths())
+    wk, wc = st.cache.attend_topk(q, st.table, st.lengths(), 6)
+    lens = st.lengths()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = st.cache.attend(q, st.table, lens)
+        gk, gc = st.cache.attend_topk(q, st.table, lens, 6)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(gk, wk) and torch.equal(gc, wc)
+
+
+def test_captured_and_replayed(kv):
+    """A step in a graph: replayed on new tokens, lengths and queries, beside eager work and a second graph."""
+    D, Hq, heads, page = 128, 8, 2, 64
+    st = Store(kv, 25, "bf16", heads, D, page, (2000, 130), width=40)
+    st.table[0, 32:] = -1
+    k, v, q = (torch.zeros(2, h, D, dtype=torch.bfloat16, device="cuda") for h in (heads, heads, Hq))
+    before, after = st.lengths(), st.lengths() + 1
+
+    def step():
+        st.cache.append(k, v, st.table, before)
+        a = st.cache.attend(q, st.table, after)
+        b, c = st.cache.attend_topk(q, st.table, after, 5)
+        return a, b, c
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs))
+    for i in range(6):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, device="cuda").to(t.dtype))
+        want = [x.clone() for x in step()]
+        torch.cuda.synchronize()
+        g, outs = graphs[i % 2]
+        for x in outs:
+            x.fill_(1)
+        g.replay()
+        junk = torch.randn(1 << 20, device="cuda").sum()  # eager work between the replays
+        torch.cuda.synchronize()
+        for x, y in zip(outs, want):
+            assert torch.equal(x, y), i
+        before += 1
+        after += 1
+        del junk
+
+
+def test_python_refusals(kv):
+    from gvdb import InvalidArgument
+
+    st = Store(kv, 26, "bf16", 2, 64, 32, (40, 9))
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    c, t, n = st.cache, st.table, st.lengths()
+    for bad in (lambda: c.attend(q.double(), t, n), lambda: c.attend(q[:, :3], t, n), lambda: c.attend(q[..., ::2], t, n),
+                lambda: c.attend(q.cpu(), t, n), lambda: c.attend(q, t.long(), n), lambda: c.attend(q, t, n[:1]),
+                lambda: c.attend(q, t, n, cu=n), lambda: c.attend(q, t, n, out=q.float()), lambda: c.attend(q[:1], t, n),
+                lambda: c.attend(q, t, n, lse=torch.zeros(2, 3, device="cuda")), lambda: c.attend_topk(q, t, n, 0),
+                lambda: c.attend_topk(q, t, n, 2, first=2, recent=1), lambda: c.append(q[:, :2], q, t, n),
+                lambda: c.append(q[:, :2], q[:, :2].float(), t, n), lambda: c.attend(q, t.t(), n),
+                lambda: kv.KvCache(4, 2, 96), lambda: kv.KvCache.from_buffers(c.pool, c.bounds[:1], c.bound_exps)):
+        with pytest.raises((InvalidArgument, Exception)) as e:
+            bad()
+        assert "VectorDbError" in [k.__name__ for k in type(e.value).__mro__], e.value
