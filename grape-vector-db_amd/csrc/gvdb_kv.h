@@ -7,6 +7,8 @@
 
 namespace gvdb {
 
+constexpr uint32_t kMaxUnits = 2048;  // sequences or rows that a balanced launch takes
+
 struct KvCache {
     uint8_t* pool;
     int8_t* bounds;
@@ -35,11 +37,16 @@ struct AttendArgs {
     KvRows q, out;
     float* lse;
     uint32_t q_heads;
-    float scale_log2;  // scale * log2(e)
+    float scale_log2;  // |scale| * log2(e), over 0
+    int32_t negate;    // scale < 0: the queries change sign
     int32_t causal;
     uint32_t row_tiles;        // tiles of query rows in the grid, a sequence (chosen pages: a token)
     uint32_t splits, chunk;    // parts along the keys, and the tiles of each
-    float *part_o, *part_ml;   // [rows][q_heads][splits][D], [..][2]
+    // the line: `lanes` waves (four a workgroup) a key head share the tiles of `units` units evenly; a unit is 16 rows (slot_rows: fewer,
+    // where a sequence or token has fewer) of a sequence, or, over chosen pages, of a token: row_tiles units each
+    uint32_t units, lanes, least, slot_rows;  // lanes = 0: one workgroup a tile of rows and split
+    uint32_t* prefix;          // [units + 1]: tiles before each unit, left for the join
+    float *part_o, *part_ml;   // [rows][q_heads][splits][D]; the line: [heads][lanes + units][slot_rows][D]; and [..][2]
     // chosen pages
     uint32_t top, first, recent, score_chunk;
     int32_t* chosen;           // [rows][heads][top]

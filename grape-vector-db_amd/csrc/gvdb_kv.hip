@@ -32,6 +32,8 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -1e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
+// Pieces of 8 bits that a type's values are split into for the products.
+constexpr int pieces(int dtype) { return dtype == GVDB_BF16 ? 1 : dtype == GVDB_F16 ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float bits_f32(uint32_t u) { return __uint_as_float(u); }
@@ -386,42 +388,101 @@ __device__ __forceinline__ uint32_t byte_bf16(const u4 (&v)[N], int b, float s) 
     }
 }
 
-// One wave's state: R tiles of 16 query rows, lane 16 q + n with row n of each.
-template <int D, int NP, int R>
-struct Rows {
-    u4 qf[R][NP][D / 32];  // query pieces, as the second operand
-    f4 o[R][D / 16];       // O^T: lane's channels q D/4 + r D/16 + j
-    float m[R], l[R];      // largest exponent (base 2) of the row; this lane's share of the sum
+// Tiles that a query at `limit` visible tokens reads: one tile beyond the table stands for a length that the
+// table does not cover, and poisons the row.
+__device__ __forceinline__ uint32_t tiles_of(const KvCache& c, const KvBatch& bt, int64_t limit) {
+    const int64_t have = (int64_t)bt.table_width * (c.page >> 5);
+    const int64_t want = limit <= 0 ? 0 : (limit + 31) >> 5;
+    return (uint32_t)min(want, have + 1);
+}
+
+// 16 query rows of a unit (a sequence; CHOSEN: one token) and key head.
+template <bool CHOSEN>
+struct Job {
+    uint32_t b, h, group;
+    int r0, n, first, rows;  // the sequence's rows of q; the first row of the 16 and the unit's rows, counted over the group's heads
+    int unit;
+    int64_t most, least;     // tokens that the last and the first of the 16 see
+    // this lane's row
+    int token;               // row of q; -1: none
+    uint32_t head;
+    int64_t limit;           // tokens that it sees
+
+    // false: no sequence has the unit
+    __device__ __forceinline__ bool set(const KvCache& c, const KvBatch& bt, const AttendArgs& a, uint32_t u, uint32_t row_tile, uint32_t hh,
+                                        uint32_t n16) {
+        unit = (int)u, b = u, h = hh, group = a.q_heads / c.heads;
+        if (CHOSEN && !a.row_seq(bt, unit, b)) return false;
+        seq_rows(bt, b, r0, n);
+        const int64_t len = max(bt.lengths[b], 0);
+        rows = (CHOSEN ? 1 : n) * (int)group;
+        first = (int)row_tile * 16;
+        const int rr = first + (int)n16;
+        token = rr < rows ? token_of(rr) : -1;
+        head = head_of(rr);
+        const int64_t before = len - n - r0 + 1;  // a token's limit, less its row
+        limit = token < 0 ? 0 : a.causal ? before + token : len;
+        most = a.causal ? before + token_of(min(first + 15, rows - 1)) : len;
+        least = a.causal ? before + token_of(first) : len;
+        return true;
+    }
+    __device__ __forceinline__ int token_of(int row) const { return CHOSEN ? unit : r0 + row / (int)group; }
+    __device__ __forceinline__ uint32_t head_of(int row) const { return h * group + (uint32_t)row % group; }
+    // Tiles that the 16 rows read.
+    __device__ __forceinline__ uint32_t tiles(const KvCache& c, const KvBatch& bt, const AttendArgs& a) const {
+        if (first >= rows) return 0;
+        return CHOSEN ? (uint32_t)min((int64_t)a.top, a.pages_seen(c, bt, most)) * (c.page >> 5) : tiles_of(c, bt, most);
+    }
+    __device__ __forceinline__ const int32_t* list(const KvCache& c, const AttendArgs& a) const {
+        return CHOSEN ? a.chosen + ((uint64_t)unit * c.heads + h) * a.top : nullptr;
+    }
 };
 
-// Scores of a tile, scaled to base 2: s[rt][i][r] of token 8q + 2r + i.
-template <int D, int NP, int R>
-__device__ __forceinline__ void tile_scores(const Rows<D, NP, R>& w, const Tile<D>& t, float c2, f4 (&s)[R][2]) {
+// One wave's state: 16 query rows, lane 16 q + n with row n.
+template <int D, int NP>
+struct Rows {
+    u4 qf[NP][D / 32];  // query pieces, as the second operand
+    f4 o[D / 16];       // O^T: lane's channels q D/4 + r D/16 + j
+    float m, l;         // largest exponent (base 2) of the row; this lane's share of the sum
+};
+
+// Tiles that a wave works on at a time: two, where the registers hold two and the two whose loads are in flight at two
+// waves a SIMD.  One maximum, one look at what is odd and one change of scale a step instead of a tile.
+template <int D, int NP>
+constexpr int kStep = D == 256 || NP == 3 ? 1 : 2;
+
+// Scores of a tile: s[i][r] of token 8q + 2r + i, without the scale.
+template <int D, int NP>
+__device__ __forceinline__ void tile_scores(const Rows<D, NP>& w, const Tile<D>& t, f4 (&s)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][i] = f4{0.f, 0.f, 0.f, 0.f};
+        s[i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
             const float sc = bits_f32((t.ks[D == 256 ? c / 4 : 0] >> (8 * i) & 255u) << 23);
             const int dw = i * (D / 32) + c;
             const bf8 a = as_bf8(codes_bf16(t.k[dw / 4][dw % 4], sc));
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, as_bf8(w.qf[r][p][c]), s[r][i], 0, 0, 0);
+            for (int p = 0; p < NP; ++p) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, as_bf8(w.qf[p][c]), s[i], 0, 0, 0);
         }
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[r][i][e] *= c2;
     }
 }
 
-// Scales of 255 mark groups that are not finite: the tile's scores of such keys become NaN.
-template <int D, int R>
-__device__ __forceinline__ void poison_scores(const Tile<D>& t, uint32_t lane, f4 (&s)[R][2]) {
+// Whether a byte of x is 255: the seven low bits carry where they are all ones.
+__device__ __forceinline__ uint32_t all_ones_byte(uint32_t x) { return ((x & 0x7F7F7F7Fu) + 0x01010101u) & x & 0x80808080u; }
+template <int D>
+__device__ __forceinline__ uint32_t odd_scales(const Tile<D>& t) {
+    uint32_t k = t.ks[0];
+    if constexpr (D == 256) k |= t.ks[1] << 16;
+    return all_ones_byte(k) | all_ones_byte(t.vs[0]) | all_ones_byte(t.vs[1]);
+}
+
+// What a tile needs where it is not wholly seen by all 16 rows, or holds what is not finite, or is not there:
+// scores of keys that are not finite become NaN and those that a row does not see -inf; rows that see a value that is not
+// finite become NaN in that value's channels; and the scales that are left are numbers.
+template <int D, int NP, bool CHOSEN>
+__device__ __forceinline__ void settle_tile(Rows<D, NP>& w, Tile<D>& t, f4 (&s)[2], const Job<CHOSEN>& j, bool there, int64_t base,
+                                            uint32_t lane) {
     const uint32_t q = lane >> 4;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -432,72 +493,43 @@ __device__ __forceinline__ void poison_scores(const Tile<D>& t, uint32_t lane, f
         b |= b >> 32;
         b |= b >> 16;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (b >> (4 * q + e) & 1u) {
+        for (int e = 0; e < 4; ++e) {
+            if (!there || (b >> (4 * q + e) & 1u)) s[i][e] = __builtin_nanf("");
+            if (base + 8 * q + 2 * e + i >= j.limit) s[i][e] = -INFINITY;
+        }
+    }
+    const int64_t seen = there ? j.most - base : 0;  // tokens behind are seen by no row: their scales may be anything
+    uint32_t badbits = 0;
+    u2 vs = t.vs;
 #pragma unroll
-                for (int r = 0; r < R; ++r) s[r][i][e] = __builtin_nanf("");
-            }
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t byte = vs[e / 4] >> (8 * (e % 4)) & 255u;
+        const bool drop = (int64_t)(8 * q + e) >= seen;
+        if (!drop && byte == 255u) badbits |= 1u << e;
+        if (drop || byte == 255u) vs[e / 4] = (vs[e / 4] & ~(255u << (8 * (e % 4)))) | 127u << (8 * (e % 4));
+    }
+    t.vs = vs;
+    if (__ballot(badbits != 0)) {  // which rows see such a value: a product of truth values
+        u4 bf, sf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            bf[r] = ((badbits >> (2 * r) & 1u) ? 0x3F80u : 0u) | ((badbits >> (2 * r + 1) & 1u) ? 0x3F800000u : 0u);
+            sf[r] = (s[0][r] != -INFINITY ? 0x3F80u : 0u) | (s[1][r] != -INFINITY ? 0x3F800000u : 0u);
+        }
+        const f4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(bf), as_bf8(sf), f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) w.o[k][e] = count[e] > 0.f ? __builtin_nanf("") : w.o[k][e];
     }
 }
 
-// Adds a tile's values by the probabilities of its scores (already masked: -inf where a row does not see a token).
-// `gone`: the tile's first token that no row sees (32: none); its scales are not read as numbers.
-template <int D, int NP, int R>
-__device__ __forceinline__ void tile_values(Rows<D, NP, R>& w, Tile<D>& t, f4 (&s)[R][2], uint32_t lane, int gone) {
-    const uint32_t q = lane >> 4;
-    u4 pf[R][NP];
-    bool seen_bad = false;
-    // scales of this lane's eight tokens
+// Adds a tile's values by the probabilities pf.
+template <int D, int NP>
+__device__ __forceinline__ void tile_values(Rows<D, NP>& w, const Tile<D>& t, const u4 (&pf)[NP]) {
     float vs[8];
-    uint32_t badbits = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        uint32_t b = t.vs[e / 4] >> (8 * (e % 4)) & 255u;
-        if ((int)(8 * q + e) >= gone) b = 127u;
-        if (b == 255u) badbits |= 1u << e, b = 127u;
-        vs[e] = bits_f32(b << 23);
-    }
-    seen_bad = __ballot(badbits != 0) != 0;
-    f4 count[R];
-    if (seen_bad) {  // which rows see a value group that is not finite: a product of truth values
-        u4 bf, sf;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            bf[r] = ((badbits >> (2 * r) & 1u) ? 0x3F80u : 0u) | ((badbits >> (2 * r + 1) & 1u) ? 0x3F800000u : 0u);
-#pragma unroll
-        for (int rt = 0; rt < R; ++rt) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                sf[r] = (s[rt][0][r] != -INFINITY ? 0x3F80u : 0u) | (s[rt][1][r] != -INFINITY ? 0x3F800000u : 0u);
-            count[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(bf), as_bf8(sf), f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt) {
-        float top = w.m[rt];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[rt][i][e]);
-        top = row_max(top);
-        const float a = __builtin_amdgcn_exp2f(w.m[rt] - top);
-        w.m[rt] = top;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(s[rt][0][e] - top), p1 = __builtin_amdgcn_exp2f(s[rt][1][e] - top);
-            sum += p0 + p1;
-            uint32_t pc[NP];
-            pack_pieces<NP>(p0, p1, pc);
-#pragma unroll
-            for (int p = 0; p < NP; ++p) pf[rt][p][e] = pc[p];
-        }
-        w.l[rt] = w.l[rt] * a + sum;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[rt][j][e] *= a;
-    }
+    for (int e = 0; e < 8; ++e) vs[e] = bits_f32((t.vs[e / 4] >> (8 * (e % 4)) & 255u) << 23);
 #pragma unroll
     for (int jb = 0; jb < D / 32; ++jb) {  // two channels a byte
         u4 even, odd;
@@ -509,187 +541,375 @@ __device__ __forceinline__ void tile_values(Rows<D, NP, R>& w, Tile<D>& t, f4 (&
             odd[r] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
 #pragma unroll
-        for (int rt = 0; rt < R; ++rt)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                w.o[rt][2 * jb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(even), as_bf8(pf[rt][p]), w.o[rt][2 * jb], 0, 0, 0);
-                w.o[rt][2 * jb + 1] =
-                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(odd), as_bf8(pf[rt][p]), w.o[rt][2 * jb + 1], 0, 0, 0);
-            }
-    }
-    if (seen_bad) {
-#pragma unroll
-        for (int rt = 0; rt < R; ++rt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (count[rt][e] > 0.f) {
-#pragma unroll
-                    for (int j = 0; j < D / 16; ++j) w.o[rt][j][e] = __builtin_nanf("");
-                }
+        for (int p = 0; p < NP; ++p) {
+            w.o[2 * jb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(even), as_bf8(pf[p]), w.o[2 * jb], 0, 0, 0);
+            w.o[2 * jb + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(odd), as_bf8(pf[p]), w.o[2 * jb + 1], 0, 0, 0);
+        }
     }
 }
 
-// Tiles that a query at `limit` visible tokens reads: one tile beyond the table stands for a length that the
-// table does not cover, and poisons the row.
-__device__ __forceinline__ uint32_t tiles_of(const KvCache& c, const KvBatch& bt, int64_t limit) {
-    const int64_t have = (int64_t)bt.table_width * (c.page >> 5);
-    const int64_t want = limit <= 0 ? 0 : (limit + 31) >> 5;
-    return (uint32_t)min(want, have + 1);
-}
-
-// Query rows of a wave's 16-row tile: row n of the sequence is token n / group, head h * group + n % group.
-struct QRow {
-    int token;       // row of q; -1: none
-    uint32_t head;
-    int64_t limit;   // tokens that it sees
+template <int D, int NT>
+struct Step {  // tiles whose loads were issued together
+    Tile<D> t[NT];
+    bool there[NT];
+    int32_t base[NT];  // first tokens
 };
 
-// ---- attend -----------------------------------------------------------------------------
-// A workgroup takes 16 query rows of one sequence (CHOSEN: of one token) and key head and one split of the
-// keys; its four waves take the split's tiles in turn, and join their parts through LDS.  With one query
-// token a sequence the kernel reads each cached byte once: 34 D / 32 bytes a token and head bound it.
-template <int D, int T, bool CHOSEN>
-__global__ __launch_bounds__(256) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
-    constexpr int NP = T == GVDB_BF16 ? 1 : T == GVDB_F16 ? 2 : 3;
-    __shared__ float s_o[4][16][D];
-    __shared__ float s_m[4][16], s_l[4][16];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
-    const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % a.splits;
-    const uint32_t unit = blockIdx.x / c.heads / a.splits;  // (sequence, tile slot), or (token, tile slot)
-    const uint32_t slot = unit % a.row_tiles;
-    uint32_t b = unit / a.row_tiles;
-    int r0, n;
-    int chosen_row = 0;
-    if constexpr (CHOSEN) {
-        chosen_row = (int)b;
-        if (!a.row_seq(bt, chosen_row, b)) return;
+// One step for 16 rows: the running maximum and sum of a softmax over its NT * 32 tokens.
+template <int D, int NP, bool CHOSEN, int NT>
+__device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const Job<CHOSEN>& j, float c2, uint32_t lane) {
+    f4 s[NT][2];
+    uint32_t odd = 0;
+    bool plain = true;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        tile_scores<D, NP>(w, st.t[x], s[x]);
+        odd |= odd_scales(st.t[x]);
+        plain &= st.there[x] && (int64_t)st.base[x] + 32 <= j.least;
     }
-    seq_rows(bt, b, r0, n);
-    const int64_t len = max(bt.lengths[b], 0);
-    const uint32_t group = a.q_heads / c.heads;
-    const int rows_here = (CHOSEN ? 1 : n) * (int)group;
-    const uint32_t per_page = c.page >> 5;
-    for (int row_tile = (int)slot; row_tile * 16 < rows_here; row_tile += (int)a.row_tiles) {
-        const int first = row_tile * 16;
-        // this lane's row
-        const int rr = first + (int)n16;
-        QRow me;
-        me.token = rr < rows_here ? (CHOSEN ? chosen_row : r0 + rr / (int)group) : -1;
-        me.head = h * group + (uint32_t)rr % group;
-        me.limit = me.token < 0 ? 0 : a.causal ? len - n + (me.token - r0) + 1 : len;
-        const int last_token = CHOSEN ? chosen_row : r0 + min(first + 15, rows_here - 1) / (int)group;
-        const int first_token = CHOSEN ? chosen_row : r0 + first / (int)group;
-        const int64_t most = a.causal ? len - n + (last_token - r0) + 1 : len;    // of the tile's rows
-        const int64_t least = a.causal ? len - n + (first_token - r0) + 1 : len;
-        const int32_t* list = nullptr;
-        uint32_t tiles;
-        if constexpr (CHOSEN) {
-            list = a.chosen + ((uint64_t)chosen_row * c.heads + h) * a.top;
-            tiles = (uint32_t)min((int64_t)a.top, a.pages_seen(c, bt, most)) * per_page;
+    if (!plain || __ballot(odd != 0)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) settle_tile<D, NP>(w, st.t[x], s[x], j, st.there[x], st.base[x], lane);
+    }
+    float top = s[0][0][0];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[x][i][e]);
+    top = fmaxf(w.m, row_max(top) * c2);
+    if (__ballot(top > w.m)) {  // some row has a new largest score: rare once a context is long
+        const float a = __builtin_amdgcn_exp2f(w.m - top);
+        w.m = top;
+        w.l *= a;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[k][e] *= a;
+    }
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        u4 pf[NP];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][0][e], c2, -top));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][1][e], c2, -top));
+            w.l += p0 + p1;
+            uint32_t pc[NP];
+            pack_pieces<NP>(p0, p1, pc);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pf[p][e] = pc[p];
+        }
+        tile_values<D, NP>(w, st.t[x], pf);
+    }
+}
+
+// Where a wave's next 64 tiles lie: lane i keeps the i-th of them, so that no tile's loads wait for the page table.
+template <bool CHOSEN>
+struct Feed {
+    uint32_t lo, hi;  // the tile's number in the pool; hi = ~0: its page is not there
+    int32_t pos;      // its first token
+
+    __device__ __forceinline__ void none() { lo = 0, hi = ~0u, pos = 0x7FFFFFFF; }
+    // Tile t of sequence b (CHOSEN: of the `top` pages in `list`).
+    __device__ __forceinline__ void take(const KvCache& c, const KvBatch& bt, uint32_t b, uint32_t h, const int32_t* list, uint32_t top,
+                                         uint32_t t) {
+        const uint32_t per_page = c.page >> 5;
+        uint32_t pj = t / per_page;
+        const uint32_t sub = t % per_page;
+        if constexpr (CHOSEN) pj = pj < top ? (uint32_t)list[pj] : ~0u;
+        pos = (int32_t)min((uint64_t)pj * c.page + sub * 32u, (uint64_t)0x7FFFFFFF);
+        const int64_t page = page_of(c, bt, b, pj);
+        if (page < 0) return;
+        const uint64_t u = ((uint64_t)page * c.heads + h) * per_page + sub;
+        lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+    }
+    // The loads of the step whose first tile is the i-th.  A tile that is not there is read as the pool's first, and not used.
+    template <int D, int NT>
+    __device__ __forceinline__ void load(const KvCache& c, uint32_t i, uint32_t lane, Step<D, NT>& st) const {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            const uint32_t l = __builtin_amdgcn_readlane(lo, i + x), u = __builtin_amdgcn_readlane(hi, i + x);
+            st.there[x] = u != ~0u;
+            st.base[x] = (int32_t)__builtin_amdgcn_readlane((uint32_t)pos, i + x);
+            load_tile<D>(c.pool + (st.there[x] ? (uint64_t)u << 32 | l : 0) * (uint64_t)(34 * D), lane, st.t[x]);
+        }
+    }
+};
+
+// A lane's part of its row of q as it lies in memory, so that its loads need not be waited for where they are issued.
+template <int D, int T>
+struct RawQueries {
+    static constexpr int N = T == GVDB_F32 ? 2 : 1;  // dwordx4 to eight channels
+    u4 r[D / 32 * N];
+
+    template <bool CHOSEN>
+    __device__ __forceinline__ void load(const AttendArgs& a, const Job<CHOSEN>& j, uint32_t q4) {
+#pragma unroll
+        for (int i = 0; i < D / 32 * N; ++i) r[i] = u4{0, 0, 0, 0};
+        if (j.token < 0) return;
+        const int64_t at = (int64_t)j.token * a.q.row_stride + (int64_t)j.head * a.q.head_stride + q4 * (D / 4);
+        if (a.q.wide) {
+            const u4* p = (const u4*)((const char*)a.q.p + at * (T == GVDB_F32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < D / 32 * N; ++i) r[i] = p[i];
+        } else if constexpr (T == GVDB_F32) {
+            const uint32_t* p = (const uint32_t*)a.q.p + at;
+#pragma unroll
+            for (int i = 0; i < D / 32 * N * 4; ++i) r[i / 4][i % 4] = p[i];
         } else {
-            tiles = tiles_of(c, bt, most);
+            const uint16_t* p = (const uint16_t*)a.q.p + at;
+#pragma unroll
+            for (int i = 0; i < D / 32 * 4; ++i) r[i / 4][i % 4] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
         }
-        const uint32_t t0 = min(split * a.chunk, tiles), t1 = split + 1 == a.splits ? tiles : min(t0 + a.chunk, tiles);
-        if (a.splits > 1 && t0 >= t1) continue;  // no part: k_kv_combine does not read it
-        Rows<D, NP, 1> w;
+    }
+    // The pieces that the products take.
+    template <int NP>
+    __device__ __forceinline__ void split(bool negate, u4 (&qf)[NP][D / 32]) const {
+        const uint32_t sign = negate ? (T == GVDB_F32 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) w.o[0][j] = f4{0.f, 0.f, 0.f, 0.f};
-        w.m[0] = kLowest;
-        w.l[0] = 0.f;
-        if (t0 < t1) {
-#pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (me.token >= 0)
-                    load8<T>(a.q.p, (int64_t)me.token * a.q.row_stride + (int64_t)me.head * a.q.head_stride + q4 * (D / 4) + 8 * ch,
-                             a.q.wide, x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t pc[NP];
-                    pack_pieces<NP>(x[2 * e], x[2 * e + 1], pc);
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) w.qf[0][p][ch][e] = pc[p];
-                }
-            }
-        }
-        for (uint32_t t = t0 + wave; t < t1; t += 4) {
-            uint32_t pj = t / per_page;
-            if constexpr (CHOSEN) pj = (uint32_t)list[pj];
-            const int64_t page = page_of(c, bt, b, pj);
-            const int64_t base = (int64_t)pj * c.page + (t % per_page) * 32;
-            if (CHOSEN && base >= most) continue;
-            Tile<D> tl;
-            load_tile<D>(c.pool + tile_at<D>(c, max(page, (int64_t)0), h, t % per_page), lane, tl);
-            f4 s[1][2];
-            tile_scores<D, NP, 1>(w, tl, a.scale_log2, s);
-            bool bad = (tl.ks[0] & 255u) == 255u || (tl.ks[0] >> 8) == 255u;
-            if constexpr (D == 256) bad |= (tl.ks[1] & 255u) == 255u || (tl.ks[1] >> 8) == 255u;
-            if (__ballot(bad)) poison_scores<D, 1>(tl, lane, s);
-            int gone = 32;
-            if (page < 0) {
-                gone = 0;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) s[0][i] = f4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
-            }
-            if (base + 32 > least || me.token < 0) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (base + 8 * q4 + 2 * e + i >= me.limit) s[0][i][e] = -INFINITY;
-                gone = (int)min((int64_t)gone, most - base);
-            }
-            tile_values<D, NP, 1>(w, tl, s, lane, gone);
-        }
-        // join the four waves
-        w.l[0] = row_sum(w.l[0]);
-        if (q4 == 0) s_m[wave][n16] = w.m[0], s_l[wave][n16] = w.l[0];
-        __syncthreads();
-        const float top = fmaxf(fmaxf(s_m[0][n16], s_m[1][n16]), fmaxf(s_m[2][n16], s_m[3][n16]));
-        const float f = __builtin_amdgcn_exp2f(w.m[0] - top);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) s_o[wave][n16][q4 * (D / 4) + r * (D / 16) + j] = w.o[0][j][r] * f;
-        __syncthreads();
-        for (uint32_t e = threadIdx.x; e < 16 * (D / 8); e += 256) {
-            const uint32_t r = e / (D / 8), d = e % (D / 8) * 8;
-            const int row = first + (int)r;
-            if (row >= rows_here) continue;
-            const int token = CHOSEN ? chosen_row : r0 + row / (int)group;
-            const uint32_t head = h * group + (uint32_t)row % group;
-            const float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-            float l = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) l += s_l[k][r] * __builtin_amdgcn_exp2f(s_m[k][r] - m);
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = (s_o[0][r][d + i] + s_o[1][r][d + i]) + (s_o[2][r][d + i] + s_o[3][r][d + i]);
-            const uint64_t at = (uint64_t)token * a.q_heads + head;
-            if (a.splits > 1) {
-                float* po = a.part_o + (at * a.splits + split) * D + d;
-                *(f4*)po = f4{x[0], x[1], x[2], x[3]};
-                *(f4*)(po + 4) = f4{x[4], x[5], x[6], x[7]};
-                if (d == 0) *(f2*)(a.part_ml + (at * a.splits + split) * 2) = f2{m, l};
+        for (int i = 0; i < D / 32 * 4; ++i) {
+            uint32_t pc[NP];
+            if constexpr (T == GVDB_BF16) {
+                pc[0] = r[i / 4][i % 4] ^ sign;
+            } else if constexpr (T == GVDB_F16) {
+                const uint32_t w = r[i / 4][i % 4] ^ sign;
+                pack_pieces<NP>((float)__builtin_bit_cast(_Float16, (uint16_t)w), (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)), pc);
             } else {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= inv;
-                store8<T>(a.out.p, (int64_t)token * a.out.row_stride + (int64_t)head * a.out.head_stride + d, a.out.wide, x);
-                if (a.lse && d == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) / kLog2e;
+                pack_pieces<NP>(bits_f32(r[i / 2][i % 2 * 2] ^ sign), bits_f32(r[i / 2][i % 2 * 2 + 1] ^ sign), pc);
             }
+#pragma unroll
+            for (int p = 0; p < NP; ++p) qf[p][i / 4][i % 4] = pc[p];
         }
+    }
+};
+
+template <int D, int NP>
+__device__ __forceinline__ void clear(Rows<D, NP>& w) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) w.o[j] = f4{0.f, 0.f, 0.f, 0.f};
+    w.m = kLowest;
+    w.l = 0.f;
+}
+
+template <int D>
+struct JoinLds {
+    float o[4][16][D], m[4][16], l[4][16];
+};
+
+// A row's output: sums over the row's keys, or over a part of them (`part`: its place among the parts).
+template <int D, int T, bool CHOSEN>
+__device__ __forceinline__ void write_row(const AttendArgs& a, const Job<CHOSEN>& j, int row, uint32_t d, float (&x)[8], float m, float l,
+                                          bool parted, uint64_t part) {
+    if (parted) {
+        float* po = a.part_o + part * D + d;
+        *(f4*)po = f4{x[0], x[1], x[2], x[3]};
+        *(f4*)(po + 4) = f4{x[4], x[5], x[6], x[7]};
+        if (d == 0) *(f2*)(a.part_ml + part * 2) = f2{m, l};
+        return;
+    }
+    const int token = j.token_of(row);
+    const uint32_t head = j.head_of(row);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= inv;
+    store8<T>(a.out.p, (int64_t)token * a.out.row_stride + (int64_t)head * a.out.head_stride + d, a.out.wide, x);
+    if (a.lse && d == 0) a.lse[(uint64_t)token * a.q_heads + head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) / kLog2e;
+}
+
+// Joins the four waves' parts of 16 rows and writes them.
+template <int D, int T, int NP, bool CHOSEN>
+__device__ __forceinline__ void join_waves(JoinLds<D>& s, Rows<D, NP>& w, const Job<CHOSEN>& j, const AttendArgs& a, uint32_t split) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, q4 = lane >> 4, n16 = lane & 15u;
+    w.l = row_sum(w.l);
+    if (q4 == 0) s.m[wave][n16] = w.m, s.l[wave][n16] = w.l;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(s.m[0][n16], s.m[1][n16]), fmaxf(s.m[2][n16], s.m[3][n16]));
+    const float f = __builtin_amdgcn_exp2f(w.m - top);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) s.o[wave][n16][q4 * (D / 4) + r * (D / 16) + k] = w.o[k][r] * f;
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < 16 * (D / 8); e += 256) {
+        const uint32_t r = e / (D / 8), d = e % (D / 8) * 8;
+        const int row = j.first + (int)r;
+        if (row >= j.rows) continue;
+        const float m = fmaxf(fmaxf(s.m[0][r], s.m[1][r]), fmaxf(s.m[2][r], s.m[3][r]));
+        float l = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) l += s.l[k][r] * __builtin_amdgcn_exp2f(s.m[k][r] - m);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (s.o[0][r][d + i] + s.o[1][r][d + i]) + (s.o[2][r][d + i] + s.o[3][r][d + i]);
+        write_row<D, T>(a, j, row, d, x, m, l, a.splits > 1,
+                        ((uint64_t)j.token_of(row) * a.q_heads + j.head_of(row)) * a.splits + split);
+    }
+    __syncthreads();
+}
+
+// Writes one wave's rows from its registers; `part`: the place of the first row's part.
+template <int D, int T, int NP, bool CHOSEN>
+__device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j, const AttendArgs& a, bool parted, uint64_t part,
+                                           uint32_t lane) {
+    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
+    const float l = row_sum(w.l);
+    if (j.token < 0) return;
+#pragma unroll
+    for (int c = 0; c < D / 4; c += 8) {  // the lane's channels: r * (D / 16) + k behind q4 * (D / 4)
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = w.o[(c + i) % (D / 16)][(c + i) / (D / 16)];
+        write_row<D, T>(a, j, j.first + (int)n16, q4 * (D / 4) + c, x, w.m, l, parted, part + n16);
+    }
+}
+
+// ---- attend -----------------------------------------------------------------------------
+// A workgroup takes 16 query rows of a unit and key head and one split of its tiles; its four waves take steps of them in
+// turn, one step's loads in flight while another is worked on, and join their parts through LDS.  With one query token a
+// sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it.
+template <int D, int T, bool CHOSEN>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
+    constexpr int NP = pieces(T), NT = kStep<D, NP>;
+    __shared__ JoinLds<D> s;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % a.splits;
+    const uint32_t rest = blockIdx.x / c.heads / a.splits;
+    for (uint32_t row_tile = rest % a.row_tiles;; row_tile += a.row_tiles) {
+        Job<CHOSEN> j;
+        if (!j.set(c, bt, a, rest / a.row_tiles, row_tile, h, lane & 15u) || j.first >= j.rows) return;
+        const uint32_t steps = (j.tiles(c, bt, a) + NT - 1) / NT, chunk = a.chunk / NT;
+        const uint32_t s0 = (uint32_t)min((uint64_t)split * chunk, (uint64_t)steps);
+        const uint32_t s1 = split + 1 == a.splits ? steps : min(s0 + chunk, steps);
+        if (a.splits > 1 && s0 >= s1) continue;  // no part: k_kv_combine does not read it
+        Rows<D, NP> w;
+        clear(w);
+        RawQueries<D, T> raw;
+        raw.load(a, j, lane >> 4);
+        const uint32_t mine = s0 + wave < s1 ? (s1 - s0 - wave + 3) / 4 : 0;
+        const int32_t* list = j.list(c, a);
+        Feed<CHOSEN> feed;
+        Step<D, NT> st, next;
+        auto fill = [&](uint32_t it) {
+            const uint32_t step = s0 + wave + 4 * (it + lane / NT);
+            feed.none();
+            if (step < s1) feed.take(c, bt, j.b, h, list, a.top, step * NT + lane % NT);
+        };
+        if (mine) {
+            fill(0);
+            feed.load(c, 0, lane, next);
+        }
+        raw.template split<NP>(a.negate, w.qf);
+        for (uint32_t it = 0; it < mine; ++it) {
+            st = next;
+            if (it + 1 < mine) {
+                const uint32_t i = (it + 1) % (64 / NT);
+                if (i == 0) fill(it + 1);
+                feed.load(c, i * NT, lane, next);
+            }
+            work_step<D, NP>(w, st, j, a.scale_log2, lane);
+        }
+        join_waves<D, T, NP>(s, w, j, a, split);
+    }
+}
+
+// The same for few rows, whose units would leave the card uneven: the steps of all units (16 rows each) lie end to end,
+// and wave w of a head takes the w-th of equal shares of that line, whatever the sequences' lengths are.  A unit that one
+// wave takes whole is written at once; the others' parts go to slot w + u (w and u only ever grow along the line: no two
+// parts share one) and are joined by k_kv_combine.  Waves never wait for one another, and loads run on over the borders
+// of units, the next unit's queries among them.
+template <int D, int T, bool CHOSEN>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
+    constexpr int NP = pieces(T), NT = kStep<D, NP>;
+    __shared__ uint32_t s_wsum[4], s_pref[kMaxUnits + 1];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t h = blockIdx.x % c.heads, w_id = blockIdx.x / c.heads * 4 + wave;
+    {
+        const uint32_t per = (a.units + 255) / 256, u0 = min(threadIdx.x * per, a.units), u1 = min(u0 + per, a.units);
+        uint32_t sum = 0;
+        for (uint32_t u = u0; u < u1; ++u) {
+            s_pref[u] = sum;
+            Job<CHOSEN> j;
+            if (j.set(c, bt, a, u / a.row_tiles, u % a.row_tiles, h, 0)) sum += (j.tiles(c, bt, a) + NT - 1) / NT;
+        }
+        uint32_t total;
+        const uint32_t before = block_scan_u32(sum, s_wsum, &total);
+        for (uint32_t u = u0; u < u1; ++u) s_pref[u] += before;
+        if (threadIdx.x == 0) s_pref[a.units] = total;
         __syncthreads();
+        if (blockIdx.x == 0)
+            for (uint32_t u = threadIdx.x; u <= a.units; u += 256) a.prefix[u] = s_pref[u];
+    }
+    const uint32_t total = s_pref[a.units], share = max(a.least / NT, (total + a.lanes - 1) / a.lanes);
+    const uint32_t at = (uint32_t)min((uint64_t)w_id * share, (uint64_t)total), end = min(at + share, total);
+    if (at >= end) return;
+    // the unit that holds a step of the line
+    auto unit_of = [&](uint32_t t) {
+        uint32_t lo = 0, hi = a.units;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (s_pref[mid + 1] <= t) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo;
+    };
+    uint32_t u = __builtin_amdgcn_readfirstlane(unit_of(at));
+    Job<CHOSEN> j, jn;
+    RawQueries<D, T> raw;
+    (void)j.set(c, bt, a, u / a.row_tiles, u % a.row_tiles, h, lane & 15u);
+    raw.load(a, j, lane >> 4);
+    Feed<CHOSEN> feed;
+    auto fill = [&](uint32_t it) {
+        const uint32_t step = at + it + lane / NT;
+        feed.none();
+        if (step >= end) return;
+        const uint32_t v = unit_of(step);
+        Job<CHOSEN> f;
+        f.unit = (int)(v / a.row_tiles), f.h = h, f.b = (uint32_t)f.unit;
+        if (!CHOSEN || a.row_seq(bt, f.unit, f.b)) feed.take(c, bt, f.b, h, f.list(c, a), a.top, (step - s_pref[v]) * NT + lane % NT);
+    };
+    Step<D, NT> st, next;
+    fill(0);
+    feed.load(c, 0, lane, next);
+    Rows<D, NP> w;
+    raw.template split<NP>(a.negate, w.qf);
+    const uint32_t mine = end - at;
+    for (uint32_t it = 0;;) {
+        const uint32_t p0 = s_pref[u], p1 = s_pref[u + 1], to = min(end, p1);
+        uint32_t v = u + 1;
+        if (to < end) {
+            while (s_pref[v + 1] <= to) ++v;  // units without tiles are left to the join
+            v = __builtin_amdgcn_readfirstlane(v);
+            (void)jn.set(c, bt, a, v / a.row_tiles, v % a.row_tiles, h, lane & 15u);
+            raw.load(a, jn, lane >> 4);
+        }
+        clear(w);
+        for (; it < to - at; ++it) {
+            st = next;
+            if (it + 1 < mine) {
+                const uint32_t i = (it + 1) % (64 / NT);
+                if (i == 0) fill(it + 1);
+                feed.load(c, i * NT, lane, next);
+            }
+            work_step<D, NP>(w, st, j, a.scale_log2, lane);
+        }
+        write_wave<D, T, NP>(w, j, a, !(at <= p0 && to == p1), ((uint64_t)h * (a.lanes + a.units) + w_id + u) * a.slot_rows, lane);
+        if (to >= end) return;
+        u = v;
+        j = jn;
+        raw.template split<NP>(a.negate, w.qf);
     }
 }
 
 // ---- combine ----------------------------------------------------------------------------
-// D / 8 threads join one row's parts: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// A wave joins one row's parts: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 8 lanes hold the channels, the
+// 512 / D groups of them take every so many-th part; the order of the sum is the lanes', alike on every run.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, AttendArgs a) {
-    const uint64_t at = (uint64_t)blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8);
-    const uint32_t d = threadIdx.x % (D / 8) * 8;
+    constexpr uint32_t L = D / 8, G = 64 / L;
+    const uint32_t lane = threadIdx.x & 63u, g = lane / L, d = lane % L * 8;
+    const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= (uint64_t)bt.rows * a.q_heads) return;
     const int token = (int)(at / a.q_heads);
     const uint32_t head = at % a.q_heads;
@@ -697,26 +917,54 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
     if (!a.row_seq(bt, token, b)) return;
     int r0, n;
     seq_rows(bt, b, r0, n);
-    const int64_t len = max(bt.lengths[b], 0);
-    const int64_t limit = a.causal ? len - n + (token - r0) + 1 : len;
-    const uint32_t tiles = CHOSEN ? (uint32_t)min((int64_t)a.top, a.pages_seen(c, bt, limit)) * (c.page >> 5) : tiles_of(c, bt, limit);
-    const uint32_t parts = min(a.splits, (tiles + a.chunk - 1) / a.chunk);
+    uint64_t first, step;  // where the parts lie
+    uint32_t parts;
+    if (a.lanes > 0) {
+        const uint32_t group = a.q_heads / c.heads;
+        const uint32_t row = (CHOSEN ? 0u : (uint32_t)(token - r0)) * group + head % group;
+        const uint32_t u = (CHOSEN ? (uint32_t)token : b) * a.row_tiles + row / 16;
+        const uint32_t p0 = a.prefix[u], p1 = a.prefix[u + 1], total = a.prefix[a.units];
+        const uint32_t share = max(a.least / kStep<D, pieces(T)>, (total + a.lanes - 1) / a.lanes);
+        const uint32_t w0 = p0 / share, w1 = p1 > p0 ? (p1 - 1) / share : w0;
+        if (p1 > p0 && w0 == w1) return;  // one workgroup took it whole
+        parts = p1 > p0 ? w1 - w0 + 1 : 0;
+        step = a.slot_rows;
+        first = ((uint64_t)(head / group) * (a.lanes + a.units) + w0 + u) * a.slot_rows + row % 16;
+    } else {
+        const int64_t len = max(bt.lengths[b], 0);
+        const int64_t limit = a.causal ? len - n + (token - r0) + 1 : len;
+        const uint32_t tiles = CHOSEN ? (uint32_t)min((int64_t)a.top, a.pages_seen(c, bt, limit)) * (c.page >> 5) : tiles_of(c, bt, limit);
+        parts = min(a.splits, (tiles + a.chunk - 1) / a.chunk);
+        step = 1;
+        first = at * a.splits;
+    }
     float m = kLowest;
-    for (uint32_t s = 0; s < parts; ++s) m = fmaxf(m, a.part_ml[(at * a.splits + s) * 2]);
-    float l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s = 0; s < parts; ++s) {
-        const f2 ml = *(const f2*)(a.part_ml + (at * a.splits + s) * 2);
-        const float f = __builtin_amdgcn_exp2f(ml[0] - m);
-        const float* po = a.part_o + (at * a.splits + s) * D + d;
+    for (uint32_t s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[(first + s * step) * 2]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t s = g; s < parts; s += G) {
+        const uint64_t p = first + s * step;
+        const f2 ml = *(const f2*)(a.part_ml + p * 2);
+        const float* po = a.part_o + p * D + d;
         const f4 u = *(const f4*)po, v = *(const f4*)(po + 4);
+        const float f = __builtin_amdgcn_exp2f(ml[0] - m);
         l += ml[1] * f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += u[i] * f, x[4 + i] += v[i] * f;
+        for (int i = 0; i < 4; ++i) o[i] += u[i] * f, o[4 + i] += v[i] * f;
     }
+#pragma unroll
+    for (uint32_t x = L; x < 64; x <<= 1) {
+        l += __shfl_xor(l, (int)x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += __shfl_xor(o[i], (int)x);
+    }
+    if (g) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= inv;
-    store8<T>(a.out.p, (int64_t)token * a.out.row_stride + (int64_t)head * a.out.head_stride + d, a.out.wide, x);
+    for (int i = 0; i < 8; ++i) o[i] *= inv;
+    store8<T>(a.out.p, (int64_t)token * a.out.row_stride + (int64_t)head * a.out.head_stride + d, a.out.wide, o);
     if (a.lse && d == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) / kLog2e;
 }
 
@@ -922,13 +1170,16 @@ hipError_t launch_kv_read(const KvCache& c, const KvBatch& bt, const KvRows& k, 
 }
 
 hipError_t launch_kv_attend(const KvCache& c, const KvBatch& bt, const AttendArgs& a, hipStream_t s) {
-    const uint64_t blocks = (uint64_t)c.heads * a.splits * a.row_tiles * bt.n_seqs;
-    const uint32_t per = 256 / (c.dim / 8);
-    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + per - 1) / per;
+    const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.n_seqs);
+    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + 3) / 4;
     if (!fits(blocks) || !fits(joins)) return hipErrorInvalidValue;
-    KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, false><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    if (a.lanes) {
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend_line<D, T, false><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    } else {
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, false><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    }
     GVDB_LAUNCH_CHECK();
-    if (a.splits > 1) {
+    if (a.lanes || a.splits > 1) {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, false><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
         GVDB_LAUNCH_CHECK();
     }
@@ -941,17 +1192,20 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
     const uint32_t chunks = (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
     const uint64_t others = (uint64_t)c.heads * chunks * bt.n_seqs;
     const uint32_t tok_tiles = capped(((uint64_t)bt.max_new + per - 1) / per, others, 1u << 22);
-    const uint64_t blocks = (uint64_t)c.heads * a.splits * a.row_tiles * bt.rows;
-    const uint32_t pb = 256 / (c.dim / 8);
-    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + pb - 1) / pb;
+    const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.rows);
+    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + 3) / 4;
     if (!fits(others * tok_tiles) || !fits(blocks) || !fits(joins) || !fits((uint64_t)bt.rows * c.heads)) return hipErrorInvalidValue;
     KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));
     GVDB_LAUNCH_CHECK();
     k_kv_select<<<bt.rows * c.heads, 256, 0, s>>>(c, bt, a);
     GVDB_LAUNCH_CHECK();
-    KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    if (a.lanes) {
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend_line<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    } else {
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    }
     GVDB_LAUNCH_CHECK();
-    if (a.splits > 1) {
+    if (a.lanes || a.splits > 1) {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
         GVDB_LAUNCH_CHECK();
     }

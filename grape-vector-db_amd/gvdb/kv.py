@@ -14,12 +14,17 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional, Tuple
 
 from . import InvalidArgument, InvalidVectorDimension, _ffi, check
 from ._ffi import lib
 
 __all__ = ["KvCache"]
+
+# struct gvdb_kv_rows and struct gvdb_kv_batch of include/gvdb.h
+_ROWS = struct.Struct("@PqqII").pack
+_BATCH = struct.Struct("@PQIIPPIIII").pack
 
 
 class KvCache:
@@ -73,52 +78,65 @@ class KvCache:
         self._lib = lib()
         self._torch = torch
         self._codes = {torch.float32: _ffi.GVDB_F32, torch.float16: _ffi.GVDB_F16, torch.bfloat16: _ffi.GVDB_BF16}
+        self._i32, self._index, self._raw_stream = torch.int32, pool.get_device(), torch._C._cuda_getCurrentRawStream
+        self._scale, self._sizes = 1.0 / math.sqrt(self.head_dim), {}
         self._c = _ffi.gvdb_kv_cache(pool.data_ptr(), bounds.data_ptr(), bound_exps.data_ptr(), n, h, self.head_dim,
-                                     self.page_size, self.device.index or 0)
+                                     self.page_size, self._index)
         self._ref = C.byref(self._c)
 
     # -- arguments ----------------------------------------------------------
-    def _rows(self, t, what: str, heads: int, rows: int):
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise InvalidArgument(f"{what} is [{rows}, {heads}, {self.head_dim}]: got {tuple(t.shape)}")
+    # A step's calls are shorter on the device than in Python: the C structs are packed as bytes (a third of a ctypes
+    # Structure's time), and a size's scratch is asked for once.
+    def _rows(self, t, what: str, heads: int, rows: int) -> bytes:
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self.head_dim:
+            raise InvalidArgument(f"{what} is [{rows}, {heads}, {self.head_dim}]: got {tuple(shape)}")
         code = self._codes.get(t.dtype)
         if code is None:
             raise InvalidArgument(f"{what} is bf16, f16 or f32: got {t.dtype}")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise InvalidArgument(f"{what} is on {t.device}, the cache on {self.device}")
-        s = t.stride()
-        if s[2] != 1:
+        if stride[2] != 1:
             raise InvalidArgument(f"{what}'s neighbouring channels lie side by side")
-        return _ffi.gvdb_kv_rows(t.data_ptr(), s[0], s[1], code, 0)
+        return _ROWS(t.data_ptr(), stride[0], stride[1], code, 0)
 
     def _batch(self, page_table, lengths, cu, rows: int, max_new: int, max_len: int):
-        i32, dev = self._torch.int32, self.device
-        if page_table.dim() != 2 or lengths.dim() != 1 or lengths.shape[0] != page_table.shape[0]:
+        """(struct, sizes): the sizes are all that a call's scratch goes by."""
+        i32, dev = self._i32, self._index
+        shape, stride = page_table.shape, page_table.stride()
+        if len(shape) != 2 or lengths.shape != shape[:1]:
             raise InvalidArgument("page_table is [sequences, width], lengths [sequences]")
-        n = page_table.shape[0]
-        if page_table.dtype != i32 or lengths.dtype != i32 or page_table.device != dev or lengths.device != dev:
+        n, width = shape
+        if page_table.dtype != i32 or lengths.dtype != i32 or page_table.get_device() != dev or lengths.get_device() != dev:
             raise InvalidArgument("page_table and lengths are int32 tensors on the cache's device")
-        if page_table.stride(1) != 1 or (n > 1 and lengths.stride(0) != 1):
+        if (width > 1 and stride[1] != 1) or (n > 1 and (lengths.stride(0) != 1 or stride[0] < width)):
             raise InvalidArgument("page_table's rows and lengths are contiguous")
-        if cu is not None and (cu.dim() != 1 or cu.shape[0] != n + 1 or cu.dtype != i32 or cu.device != dev or cu.stride(0) != 1):
-            raise InvalidArgument("cu is a contiguous int32 [sequences + 1] on the cache's device")
-        if max_new < 0 or max_len < 0:
-            raise InvalidArgument("max_new and max_len are not negative")
-        return _ffi.gvdb_kv_batch(page_table.data_ptr(), page_table.stride(0), page_table.shape[1], n, lengths.data_ptr(),
-                                  None if cu is None else cu.data_ptr(), rows, max_new, max_len, 0)
+        if cu is None:
+            at = 0
+        else:
+            if cu.dim() != 1 or cu.shape[0] != n + 1 or cu.dtype != i32 or cu.get_device() != dev or cu.stride(0) != 1:
+                raise InvalidArgument("cu is a contiguous int32 [sequences + 1] on the cache's device")
+            at = cu.data_ptr()
+        if max_new < 0 or max_len < 0 or max_new > 0xFFFFFFFF or max_len > 0xFFFFFFFF:
+            raise InvalidArgument("max_new and max_len are not negative, and below 2^32")
+        return (_BATCH(page_table.data_ptr(), stride[0], width, n, lengths.data_ptr(), at, rows, max_new, max_len, 0),
+                (rows, n, width, at != 0, max_new, max_len))
 
     def _stream(self, stream: Optional[int]):
         if stream is not None:
             return stream or None
-        return self._torch.cuda.current_stream(self.device).cuda_stream or None
+        return self._raw_stream(self._index) or None
 
     # -- operators ----------------------------------------------------------
     def append(self, k, v, page_table, lengths, cu=None, max_new: int = 0, stream: Optional[int] = None) -> None:
         """Writes rows ``k`` and ``v`` as tokens ``lengths[s]`` .. of each sequence (``lengths``: tokens before the call)."""
-        kr = self._rows(k, "k", self.kv_heads, k.shape[0])
-        vr = self._rows(v, "v", self.kv_heads, k.shape[0])
-        bt = self._batch(page_table, lengths, cu, k.shape[0], max_new, 0)
-        check(self._lib.gvdb_kv_append_device(self._ref, C.byref(bt), C.byref(kr), C.byref(vr), self._stream(stream)))
+        rows = k.shape[0]
+        kr = self._rows(k, "k", self.kv_heads, rows)
+        vr = self._rows(v, "v", self.kv_heads, rows)
+        bt, _ = self._batch(page_table, lengths, cu, rows, max_new, 0)
+        status = self._lib.gvdb_kv_append_device(self._ref, bt, kr, vr, self._stream(stream))
+        if status:
+            check(status)
 
     def read(self, page_table, lengths, rows: int, cu=None, max_new: int = 0, dtype=None, out=None,
              stream: Optional[int] = None) -> Tuple:
@@ -132,41 +150,50 @@ class KvCache:
             out = (make(shape, dtype=dtype, device=self.device), make(shape, dtype=dtype, device=self.device))
         kr = self._rows(out[0], "out[0]", self.kv_heads, rows)
         vr = self._rows(out[1], "out[1]", self.kv_heads, rows)
-        bt = self._batch(page_table, lengths, cu, rows, max_new, 0)
-        check(self._lib.gvdb_kv_read_device(self._ref, C.byref(bt), C.byref(kr), C.byref(vr), self._stream(stream)))
+        bt, _ = self._batch(page_table, lengths, cu, rows, max_new, 0)
+        status = self._lib.gvdb_kv_read_device(self._ref, bt, kr, vr, self._stream(stream))
+        if status:
+            check(status)
         return out
 
-    def _attend_args(self, q, page_table, lengths, cu, max_new, max_len, scale, out, lse):
+    def _attend_args(self, q, page_table, lengths, cu, max_new, max_len, scale, out, lse, top):
         torch = self._torch
-        if q.dim() != 3:
+        shape = q.shape
+        if len(shape) != 3:
             raise InvalidArgument("q is [rows, heads, head_dim]")
-        rows, heads = q.shape[0], q.shape[1]
+        rows, heads = shape[0], shape[1]
         qr = self._rows(q, "q", heads, rows)
         if out is None:
             # rows behind the last sequence are not written: without `out` they read 0
-            out = (torch.empty if cu is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q) if cu is None else torch.zeros_like(q)
         orow = self._rows(out, "out", heads, rows)
-        if lse is not None and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != self.device
+        if lse is not None and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.get_device() != self._index
                                 or not lse.is_contiguous()):
             raise InvalidArgument("lse is a contiguous float32 [rows, heads] on the cache's device")
-        bt = self._batch(page_table, lengths, cu, rows, max_new, max_len)
-        return heads, qr, orow, bt, (1.0 / math.sqrt(self.head_dim) if scale is None else scale), out
-
-    def _scratch(self, bt, heads: int, top: int):
-        n = C.c_uint64()
-        check(self._lib.gvdb_kv_scratch_bytes(self._ref, C.byref(bt), heads, top, C.byref(n)))
+        bt, sizes = self._batch(page_table, lengths, cu, rows, max_new, max_len)
+        key = (sizes, heads, top)
+        size = self._sizes.get(key)
+        if size is None:
+            n = C.c_uint64()
+            check(self._lib.gvdb_kv_scratch_bytes(self._ref, bt, heads, top, C.byref(n)))
+            if len(self._sizes) >= 4096:
+                self._sizes.clear()
+            size = self._sizes[key] = n.value
         # torch's allocator keeps it apart from other streams' and graphs' scratch
-        return self._torch.empty(n.value, dtype=self._torch.uint8, device=self.device) if n.value else None, n.value
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+        return heads, qr, orow, bt, (self._scale if scale is None else scale), out, scratch, size
 
     def attend(self, q, page_table, lengths, cu=None, max_new: int = 0, max_len: int = 0, scale: Optional[float] = None,
                causal: bool = True, out=None, lse=None, stream: Optional[int] = None):
         """Attention of rows ``q`` over their sequences' tokens (``lengths``: with the call's own).  With ``causal``, row i of a
         sequence's n sees the first ``length - n + i + 1`` tokens.  ``scale``: 1 / sqrt(head_dim) by default; ``lse``
         [rows, heads] float32 takes the logarithm of the softmax's denominator.  A row that sees nothing is 0."""
-        heads, qr, orow, bt, scale, out = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out, lse)
-        scratch, size = self._scratch(bt, heads, 0)
-        check(self._lib.gvdb_kv_attend_device(self._ref, C.byref(bt), C.byref(qr), heads, scale, int(causal), C.byref(orow),
-                                              _ffi.ptr(lse), _ffi.ptr(scratch), size, self._stream(stream)))
+        heads, qr, orow, bt, scale, out, scratch, size = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out,
+                                                                           lse, 0)
+        status = self._lib.gvdb_kv_attend_device(self._ref, bt, qr, heads, scale, 1 if causal else 0, orow, _ffi.ptr(lse),
+                                                 _ffi.ptr(scratch), size, self._stream(stream))
+        if status:
+            check(status)
         return out
 
     def attend_topk(self, q, page_table, lengths, top: int, first: int = 1, recent: int = 1, cu=None, max_new: int = 0,
@@ -176,17 +203,18 @@ class KvCache:
         those whose key bounds promise the largest scores.  Returns ``(out, chosen)``; ``chosen`` is int32 [rows, kv_heads,
         top], positions in the page table in order, -1 behind the last."""
         torch = self._torch
-        heads, qr, orow, bt, scale, out = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out, lse)
-        if top < 1 or first < 0 or recent < 0:
-            raise InvalidArgument("top is at least 1, first and recent are not negative")
+        if top < 1 or first < 0 or recent < 0 or first + recent > top:
+            raise InvalidArgument("top is at least 1 and at least first + recent, which are not negative")
+        heads, qr, orow, bt, scale, out, scratch, size = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out,
+                                                                           lse, top)
         shape = (q.shape[0], self.kv_heads, top)
         if chosen is None:
             chosen = torch.empty(shape, dtype=torch.int32, device=self.device) if cu is None else torch.full(
                 shape, -1, dtype=torch.int32, device=self.device)
-        elif tuple(chosen.shape) != shape or chosen.dtype != torch.int32 or chosen.device != self.device or not chosen.is_contiguous():
+        elif tuple(chosen.shape) != shape or chosen.dtype != torch.int32 or chosen.get_device() != self._index or not chosen.is_contiguous():
             raise InvalidArgument("chosen is a contiguous int32 [rows, kv_heads, top] on the cache's device")
-        scratch, size = self._scratch(bt, heads, top)
-        check(self._lib.gvdb_kv_attend_topk_device(self._ref, C.byref(bt), C.byref(qr), heads, scale, top, first, recent,
-                                                   C.byref(orow), chosen.data_ptr(), _ffi.ptr(lse), _ffi.ptr(scratch), size,
-                                                   self._stream(stream)))
+        status = self._lib.gvdb_kv_attend_topk_device(self._ref, bt, qr, heads, scale, top, first, recent, orow, chosen.data_ptr(),
+                                                      _ffi.ptr(lse), _ffi.ptr(scratch), size, self._stream(stream))
+        if status:
+            check(status)
         return out, chosen

@@ -248,8 +248,8 @@ def test_attend(kv, dtype, Hq, heads, D, page, lens, new):
     lse = torch.full(q.shape[:2], 5.0, device="cuda")
     out = st.cache.attend(q, st.table, st.lengths(), cu=cu, lse=lse, max_new=max(new), max_len=max(lens))
     check_attend(st, q, new, out, lse)
-    if len(set(new)) == 1:
-        assert torch.equal(out, st.cache.attend(q, st.table, st.lengths(), max_len=max(lens)))
+    if len(set(new)) == 1:  # without cu the keys may be cut elsewhere: another order of the same sums, under the same bound
+        check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), max_len=max(lens)))
     # hints size the launch only: too small, too large and none give the same sums up to their order
     for hints in ({"max_new": 1, "max_len": 1}, {}, {"max_new": 10 ** 6, "max_len": 10 ** 6}):
         check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), cu=cu, **hints))
