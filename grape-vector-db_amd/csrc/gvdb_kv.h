@@ -7,6 +7,7 @@
 
 namespace gvdb {
 
+constexpr uint32_t kChooseScores = 15360;  // page scores that a choosing workgroup keeps in LDS: two workgroups a CU
 constexpr uint32_t kMaxUnits = 2048;  // sequences or rows that a balanced launch takes
 
 struct KvCache {
@@ -31,6 +32,7 @@ struct KvRows {
     uint32_t dtype;
     int64_t row_stride, head_stride;  // elements
     bool wide;                        // base and strides are multiples of 16 bytes
+    bool zero_rest;                   // outputs: rows of no sequence become 0
 };
 
 struct AttendArgs {
@@ -40,7 +42,8 @@ struct AttendArgs {
     float scale_log2;  // |scale| * log2(e), over 0
     int32_t negate;    // scale < 0: the queries change sign
     int32_t causal;
-    uint32_t row_tiles;        // tiles of query rows in the grid, a sequence (chosen pages: a token)
+    uint32_t row_tiles;        // tiles of query rows in the grid, a sequence (chosen pages: a token): 16 rows, `many`: 128
+    bool many;
     uint32_t splits, chunk;    // parts along the keys, and the tiles of each
     // the line: `lanes` waves (four a workgroup) a key head share the tiles of `units` units evenly; a unit is 16 rows (slot_rows: fewer,
     // where a sequence or token has fewer) of a sequence, or, over chosen pages, of a token: row_tiles units each
@@ -48,7 +51,8 @@ struct AttendArgs {
     uint32_t* prefix;          // [units + 1]: tiles before each unit, left for the join
     float *part_o, *part_ml;   // [rows][q_heads][splits][D]; the line: [heads][lanes + units][slot_rows][D]; and [..][2]
     // chosen pages
-    uint32_t top, first, recent, score_chunk;
+    uint32_t top, first, recent;
+    uint32_t score_chunk;      // pages a workgroup scores into `scores`; 0: scored and chosen by one workgroup in LDS
     int32_t* chosen;           // [rows][heads][top]
     float* scores;             // [rows][heads][table_width]
 

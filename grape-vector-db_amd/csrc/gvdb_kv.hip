@@ -27,6 +27,9 @@ typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -34,6 +37,19 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kLowest = -1e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
 // Pieces of 8 bits that a type's values are split into for the products.
 constexpr int pieces(int dtype) { return dtype == GVDB_BF16 ? 1 : dtype == GVDB_F16 ? 2 : 3; }
+// The value, as one that the compiler knows nothing of: what is reckoned from it in a branch that is seldom taken stays in
+// that branch, and takes no registers outside.
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+template <int V>
+struct Const {
+    static constexpr int value = V;
+};
+// A row's sums are rescaled only when a score passes the reference by so much (base 2): probabilities reach 2^8 instead of 1,
+// which no rounding notices, and a new largest score, which some row of a wave has in half of all steps, seldom costs anything.
+constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float bits_f32(uint32_t u) { return __uint_as_float(u); }
@@ -178,28 +194,110 @@ __device__ __forceinline__ uint32_t value_byte(uint32_t t, uint32_t b) {
 
 // Eight codes as the values that they stand for.
 __device__ __forceinline__ void code_values(uint32_t w, uint32_t scale, float (&x)[8]) {
-    const float s = scale == 255u ? __builtin_nanf("") : bits_f32(scale << 23);
+    const float s = bits_f32(scale << 23);
+    const f2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const f2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+    const bool bad = scale == 255u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t c = (w >> (4 * i)) & 15u;
-        // e2m1: subnormal 0, .5, then (2 + m) * 2^(e - 2)
-        const uint32_t e = (c >> 1) & 3u, m = c & 1u;
-        const float v = e == 0 ? 0.5f * (float)m : bits_f32(((e + 126u) << 23) | (m << 22));
-        x[i] = ((c & 8u) ? -v : v) * s;
+    for (int i = 0; i < 2; ++i) {
+        x[i] = bad ? __builtin_nanf("") : v0[i], x[2 + i] = bad ? __builtin_nanf("") : v1[i];
+        x[4 + i] = bad ? __builtin_nanf("") : v2[i], x[6 + i] = bad ? __builtin_nanf("") : v3[i];
     }
 }
 
+// Largest over the lanes that differ in their lowest two bits, and over a wave.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+    x = max(x, dpp<0xB1>(x));
+    return max(x, dpp<0x4E>(x));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = quad_max(x);
+    x = max(x, dpp<0x141>(x));
+    x = max(x, dpp<0x140>(x));
+    u2 r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(r[0], r[1]);
+}
+
+// Eight neighbouring elements as they lie in memory.
+template <int T>
+struct Raw8 {
+    u4 r[T == GVDB_F32 ? 2 : 1];
+
+    __device__ __forceinline__ void load(const void* base, int64_t at, bool wide) {
+        constexpr int N = T == GVDB_F32 ? 2 : 1;
+        if (wide) {
+            const u4* p = (const u4*)((const char*)base + at * (T == GVDB_F32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = p[i];
+        } else if constexpr (T == GVDB_F32) {
+            const uint32_t* p = (const uint32_t*)base + at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i / 4][i % 4] = p[i];
+        } else {
+            const uint16_t* p = (const uint16_t*)base + at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[0][i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+        }
+    }
+    // The largest magnitude's bits as a float's: magnitudes order as their bits do, NaN above all.
+    __device__ __forceinline__ uint32_t amax() const {
+        if constexpr (T == GVDB_F32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, r[i / 4][i % 4] & 0x7FFFFFFFu);
+            return m;
+        } else {
+            us2 m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, r[0][i] & 0x7FFF7FFFu));
+            const uint16_t x = max(m[0], m[1]);
+            return T == GVDB_BF16 ? (uint32_t)x << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, x));
+        }
+    }
+    // The codes at 2^(scale - 127): the conversion rounds to nearest, ties to the even code.
+    __device__ __forceinline__ uint32_t codes(uint32_t scale) const {
+        const float s = bits_f32(scale << 23);
+        uint32_t w = 0;
+        const uint32_t x0 = r[0][0], x1 = r[0][1], x2 = r[0][2], x3 = r[0][3];  // a bit cast of a vector's element reads its first
+        if constexpr (T == GVDB_F32) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, bits_f32(x0), bits_f32(x1), s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, bits_f32(x2), bits_f32(x3), s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, bits_f32(r[1][0]), bits_f32(r[1][1]), s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, bits_f32(r[1][2]), bits_f32(r[1][3]), s, 3);
+        } else if constexpr (T == GVDB_F16) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h2, x0), s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h2, x1), s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h2, x2), s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(h2, x3), s, 3);
+        } else {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf2, x0), s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf2, x1), s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf2, x2), s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf2, x3), s, 3);
+        }
+        return w;
+    }
+};
+
 // ---- append -----------------------------------------------------------------------------
-// One workgroup a touched page, head and part (keys, values).  D / 8 threads take a token, eight channels
-// each; four neighbours share a scale.  Bound by the reads of k and v.
+// One workgroup a touched page, head and part (keys, values).  D / 8 threads take a token, eight channels each; four neighbours
+// share a scale.  Four passes' loads are in flight at once.  Bound by the reads of k and v where there are many tokens, and by
+// its chain of loads (length, page, rows) where there is one.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows k, KvRows v, uint32_t slots) {
     constexpr uint32_t TPT = D / 8;       // threads a token
     constexpr uint32_t TPB = 256 / TPT;   // tokens a pass
-    __shared__ float s_hi[TPB][D], s_lo[TPB][D];
-    __shared__ uint32_t s_bad, s_exp;
+    constexpr int AHEAD = 4;
+    __shared__ float s_hi[4][D], s_lo[4][D];
+    __shared__ uint32_t s_bad[4], s_amax[4];
     const uint32_t b = blockIdx.x / slots, part = blockIdx.y & 1u, h = blockIdx.y >> 1;
-    const uint32_t o = threadIdx.x % TPT, lane_t = threadIdx.x / TPT;
+    const uint32_t o = threadIdx.x % TPT, lane_t = threadIdx.x / TPT, wave = threadIdx.x >> 6;
     int r0, n;
     seq_rows(bt, b, r0, n);
     const int64_t start = max(bt.lengths[b], 0), end = start + n;
@@ -209,81 +307,100 @@ __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows
         if (page < 0) continue;  // the same for the whole workgroup
         const int64_t p0 = pj * c.page;
         const uint32_t lo_t = (uint32_t)max(start - p0, (int64_t)0), hi_t = (uint32_t)min(end - p0, (int64_t)c.page);
+        uint8_t* const tiles = c.pool + tile_at<D>(c, page, h, 0) + part * (17 * D);
+        auto code_at = [&](uint32_t t) { return tiles + (t >> 5) * (34 * D) + (part ? value_byte<D>(t & 31u, 4 * o) : key_byte<D>(t & 31u, o)); };
+        auto scale_at = [&](uint32_t t) { return tiles + (t >> 5) * (34 * D) + 16 * D + o / 4 * 32 + (t & 31u); };
         float hi[8], lo[8];
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
         // tokens that the page holds already count for its bounds; values have none
-        for (uint32_t t = (part ? lo_t / TPB * TPB : 0) + lane_t; t < hi_t; t += TPB) {
-            uint8_t* tile = c.pool + tile_at<D>(c, page, h, t >> 5) + part * (17 * D);
-            const uint32_t t5 = t & 31u, g = o / 4;
-            uint8_t* scales = tile + 16 * D + g * 32 + t5;
-            float x[8];
-            if (t < lo_t) {
-                if (part) continue;
-                const uint32_t w = *(const uint32_t*)(tile + key_byte<D>(t5, o));
-                const uint32_t s = *scales;
-                bad |= s == 255u;
-                code_values(w, s, x);
-            } else {
-                load8<T>(src.p, (r0 + (p0 + t - start)) * src.row_stride + (int64_t)h * src.head_stride + 8 * o, src.wide, x);
-                uint32_t amax = 0;  // magnitudes order as their bits do; NaN is the largest
+        for (uint32_t first = (part ? lo_t / TPB * TPB : 0) + lane_t; first < hi_t; first += AHEAD * TPB) {
+            Raw8<T> raw[AHEAD];
+            uint32_t w[AHEAD], s[AHEAD];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1));
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 2));
-                // 2^e, the smallest with amax < 7 * 2^e: the fraction's .75 carries into the exponent
-                uint32_t s = (amax + 0x200000u) >> 23;
-                s = min(max(s, 4u) - 2u, 252u);
-                const bool inf = amax >= 0x7F800000u;
-                const float up = bits_f32((254u - s) << 23);  // 2^(127 - s), exact
-                uint32_t w = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float y = fabsf(x[i]) * up;
-                    uint32_t code = (uint32_t)(y > 0.25f) + (y >= 0.75f) + (y > 1.25f) + (y >= 1.75f) + (y > 2.5f) +
-                                    (y >= 3.5f) + (y > 5.0f);
-                    code |= x[i] < 0.0f ? 8u : 0u;
-                    w |= code << (4 * i);
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t t = first + i * TPB;
+                w[i] = s[i] = 0;
+                if (t >= hi_t) continue;
+                if (t >= lo_t) {
+                    raw[i].load(src.p, (r0 + (p0 + t - start)) * src.row_stride + (int64_t)h * src.head_stride + 8 * o, src.wide);
+                } else if (!part) {
+                    w[i] = *(const uint32_t*)code_at(t);
+                    s[i] = *scale_at(t);
                 }
-                if (inf) w = 0, s = 255u;
-                bad |= inf;
-                if (part == 0) {
-                    *(uint32_t*)(tile + key_byte<D>(t5, o)) = w;
-                } else if constexpr (D == 64) {
-                    *(uint16_t*)(tile + value_byte<D>(t5, 4 * o)) = (uint16_t)w;
-                    *(uint16_t*)(tile + value_byte<D>(t5, 4 * o + 2)) = (uint16_t)(w >> 16);
-                } else {
-                    *(uint32_t*)(tile + value_byte<D>(t5, 4 * o)) = w;
-                }
-                if ((o & 3u) == 0) *scales = (uint8_t)s;
-                if (part) continue;
-                code_values(w, s, x);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) hi[i] = fmaxf(hi[i], x[i]), lo[i] = fminf(lo[i], x[i]);
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t t = first + i * TPB;
+                if (t >= hi_t || (part && t < lo_t)) continue;
+                if (t >= lo_t) {
+                    const uint32_t amax = quad_max(raw[i].amax());
+                    // 2^e, the smallest with amax < 7 * 2^e: the fraction's .75 carries into the exponent
+                    s[i] = min(max((amax + 0x200000u) >> 23, 4u) - 2u, 252u);
+                    w[i] = raw[i].codes(s[i]);
+                    if (amax >= 0x7F800000u) w[i] = 0, s[i] = 255u;
+                    uint8_t* to = code_at(t);
+                    if (D == 64 && part) {
+                        *(uint16_t*)to = (uint16_t)w[i];
+                        *(uint16_t*)(tiles + (t >> 5) * (34 * D) + value_byte<D>(t & 31u, 4 * o + 2)) = (uint16_t)(w[i] >> 16);
+                    } else {
+                        *(uint32_t*)to = w[i];
+                    }
+                    if ((o & 3u) == 0) *scale_at(t) = (uint8_t)s[i];
+                    if (part) continue;
+                }
+                bad |= s[i] == 255u;
+                float x[8];
+                code_values(w[i], s[i], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) hi[e] = fmaxf(hi[e], x[e]), lo[e] = fminf(lo[e], x[e]);
+            }
         }
         if (part) continue;
-        // the page's bounds: over the passes' threads, then one power of two for all channels
-        if (threadIdx.x == 0) s_bad = 0, s_exp = 0;
+        // the page's bounds: over the wave's tokens, the waves, then one power of two for all channels
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s_hi[lane_t][8 * o + i] = hi[i], s_lo[lane_t][8 * o + i] = lo[i];
-        __syncthreads();
-        if (bad) s_bad = 1;
-        const uint32_t d = threadIdx.x;
-        float h1 = -INFINITY, l1 = INFINITY;
-        if (d < D) {
-            for (uint32_t i = 0; i < TPB; ++i) h1 = fmaxf(h1, s_hi[i][d]), l1 = fminf(l1, s_lo[i][d]);
-            atomicMax(&s_exp, __float_as_uint(fmaxf(fabsf(h1), fabsf(l1))));  // LDS; the largest, in any order
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (D == 64) {  // a rotation by 8 of 16 lanes
+                hi[e] = fmaxf(hi[e], bits_f32(dpp<0x128>(__float_as_uint(hi[e]))));
+                lo[e] = fminf(lo[e], bits_f32(dpp<0x128>(__float_as_uint(lo[e]))));
+            }
+            if constexpr (D <= 128) {
+                u2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(hi[e]), __float_as_uint(hi[e]), false, false);
+                hi[e] = fmaxf(bits_f32(r[0]), bits_f32(r[1]));
+                r = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo[e]), __float_as_uint(lo[e]), false, false);
+                lo[e] = fminf(bits_f32(r[0]), bits_f32(r[1]));
+            }
+            u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(hi[e]), __float_as_uint(hi[e]), false, false);
+            hi[e] = fmaxf(bits_f32(r[0]), bits_f32(r[1]));
+            r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lo[e]), __float_as_uint(lo[e]), false, false);
+            lo[e] = fminf(bits_f32(r[0]), bits_f32(r[1]));
         }
+        const uint64_t any_bad = __ballot(bad);
+        if ((threadIdx.x & 63u) < TPT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s_hi[wave][8 * o + e] = hi[e], s_lo[wave][8 * o + e] = lo[e];
+        }
+        if ((threadIdx.x & 63u) == 0) s_bad[wave] = any_bad != 0;
+        __syncthreads();
+        const uint32_t d = threadIdx.x;
+        float h1 = 0.f, l1 = 0.f;
+        if (d < D) {
+            h1 = fmaxf(fmaxf(s_hi[0][d], s_hi[1][d]), fmaxf(s_hi[2][d], s_hi[3][d]));
+            l1 = fminf(fminf(s_lo[0][d], s_lo[1][d]), fminf(s_lo[2][d], s_lo[3][d]));
+        }
+        const uint32_t wm = wave_max(__float_as_uint(fmaxf(fabsf(h1), fabsf(l1))));
+        if ((threadIdx.x & 63u) == 0) s_amax[wave] = wm;
         __syncthreads();
         if (d < D) {
+            const bool any = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+            const uint32_t amax = max(max(s_amax[0], s_amax[1]), max(s_amax[2], s_amax[3]));
             // 2^b, the smallest with amax <= 127 * 2^b (fractions over 127/128 carry), rounded outward
-            const uint32_t e = s_bad ? 255u : min(max((s_exp + 0x1FFFFu) >> 23, 7u), 254u);
+            const uint32_t e = any ? 255u : min(max((amax + 0x1FFFFu) >> 23, 7u), 254u);
             const float up = bits_f32((260u - min(e, 254u)) << 23);  // 2^(133 - e)
             int8_t* q = c.bounds + ((uint64_t)page * c.heads + h) * (2 * D);
-            q[d] = s_bad ? (int8_t)0 : (int8_t)ceilf(h1 * up);
-            q[D + d] = s_bad ? (int8_t)0 : (int8_t)floorf(l1 * up);
+            q[d] = any ? (int8_t)0 : (int8_t)ceilf(h1 * up);
+            q[D + d] = any ? (int8_t)0 : (int8_t)floorf(l1 * up);
             if (d == 0) c.bound_exps[(uint64_t)page * c.heads + h] = (uint8_t)e;
         }
         __syncthreads();
@@ -291,17 +408,23 @@ __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows
 }
 
 // ---- read -------------------------------------------------------------------------------
-// A thread takes eight channels of one token and head, keys and values.
+// A thread takes eight channels of one token and head, keys and values; a workgroup several tokens of one head, whose codes lie
+// side by side.  Bound by what it writes.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_read(KvCache c, KvBatch bt, KvRows k, KvRows v) {
     constexpr uint32_t TPT = D / 8;
     const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t o = at % TPT;
-    const uint64_t rest = at / TPT;
+    constexpr uint32_t TPB = 256 / TPT;
+    const uint64_t rest = at / 256;
     const uint32_t h = rest % c.heads;
-    const uint64_t row = rest / c.heads;
+    const uint64_t row = rest / c.heads * TPB + at % 256 / TPT;
     if (row >= bt.rows) return;
     uint32_t b;
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto rest_of = [&](const KvRows& r) {  // behind the last sequence: left as it was, or 0
+        if (r.p && r.zero_rest) store8<T>(r.p, (int64_t)row * r.row_stride + (int64_t)h * r.head_stride + 8 * o, r.wide, zero);
+    };
     if (bt.cu) {  // the last sequence that begins at or before the row
         uint32_t lo = 0, hi = bt.n_seqs;
         while (lo < hi) {
@@ -310,13 +433,19 @@ __global__ __launch_bounds__(256) void k_kv_read(KvCache c, KvBatch bt, KvRows k
             else hi = mid;
         }
         b = lo;
-        if (b >= bt.n_seqs) return;  // behind the last sequence: left as it was
+        if (b >= bt.n_seqs) {
+            rest_of(k), rest_of(v);
+            return;
+        }
     } else {
         b = (uint32_t)(row / (bt.rows / bt.n_seqs));
     }
     int r0, n;
     seq_rows(bt, b, r0, n);
-    if ((int64_t)row < r0) return;
+    if ((int64_t)row < r0) {
+        rest_of(k), rest_of(v);
+        return;
+    }
     const int64_t pos = (int64_t)max(bt.lengths[b], 0) + ((int64_t)row - r0);
     const int64_t pj = pos / c.page;
     const int64_t page = pj < (int64_t)bt.table_width ? page_of(c, bt, b, (uint32_t)pj) : -1;
@@ -483,7 +612,7 @@ __device__ __forceinline__ uint32_t odd_scales(const Tile<D>& t) {
 template <int D, int NP, bool CHOSEN>
 __device__ __forceinline__ void settle_tile(Rows<D, NP>& w, Tile<D>& t, f4 (&s)[2], const Job<CHOSEN>& j, bool there, int64_t base,
                                             uint32_t lane) {
-    const uint32_t q = lane >> 4;
+    const uint32_t q = opaque(lane) >> 4;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         bool bad = (t.ks[0] >> (8 * i) & 255u) == 255u;
@@ -578,8 +707,10 @@ __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[x][i][e]);
-    top = fmaxf(w.m, row_max(top) * c2);
-    if (__ballot(top > w.m)) {  // some row has a new largest score: rare once a context is long
+    top = row_max(top) * c2;
+    const bool over = top > w.m + kSlack;
+    top = over ? top : w.m;
+    if (__ballot(over)) {
         const float a = __builtin_amdgcn_exp2f(w.m - top);
         w.m = top;
         w.l *= a;
@@ -595,9 +726,9 @@ __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const
         for (int e = 0; e < 4; ++e) {
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][0][e], c2, -top));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][1][e], c2, -top));
-            w.l += p0 + p1;
             uint32_t pc[NP];
             pack_pieces<NP>(p0, p1, pc);
+            w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
 #pragma unroll
             for (int p = 0; p < NP; ++p) pf[p][e] = pc[p];
         }
@@ -684,6 +815,23 @@ struct RawQueries {
         }
     }
 };
+
+// Rows of no sequence: left as they were, or (out.zero_rest) 0, their logarithm -inf and their pages -1.
+template <int D, int T>
+__device__ __forceinline__ void clear_rest(const KvCache& c, const KvBatch& bt, const AttendArgs& a) {
+    if (!a.out.zero_rest || !bt.cu) return;
+    const int from = min(max(bt.cu[bt.n_seqs], 0), (int)bt.rows), head = min(max(bt.cu[0], 0), from);
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int64_t r = blockIdx.x; r < (int64_t)bt.rows - from + head; r += gridDim.x) {
+        const int64_t row = r < head ? r : r - head + from;
+        for (uint32_t i = threadIdx.x; i < a.q_heads * (D / 8); i += blockDim.x)
+            store8<T>(a.out.p, row * a.out.row_stride + (int64_t)(i / (D / 8)) * a.out.head_stride + i % (D / 8) * 8, a.out.wide, zero);
+        if (a.lse)
+            for (uint32_t i = threadIdx.x; i < a.q_heads; i += blockDim.x) a.lse[row * a.q_heads + i] = -INFINITY;
+        if (a.top)
+            for (uint32_t i = threadIdx.x; i < c.heads * a.top; i += blockDim.x) a.chosen[row * c.heads * a.top + i] = -1;
+    }
+}
 
 template <int D, int NP>
 __device__ __forceinline__ void clear(Rows<D, NP>& w) {
@@ -773,6 +921,7 @@ template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T), NT = kStep<D, NP>;
     __shared__ JoinLds<D> s;
+    clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % a.splits;
     const uint32_t rest = blockIdx.x / c.heads / a.splits;
@@ -823,6 +972,7 @@ template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T), NT = kStep<D, NP>;
     __shared__ uint32_t s_wsum[4], s_pref[kMaxUnits + 1];
+    clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t h = blockIdx.x % c.heads, w_id = blockIdx.x / c.heads * 4 + wave;
     {
@@ -902,14 +1052,330 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
     }
 }
 
+// ---- attend, many rows ----------------------------------------------------------------
+// A workgroup takes 128 query rows of a sequence and key head and one split of the tokens, 32 rows a wave, 64 tokens a
+// step, by v_mfma_f32_32x32x16_bf16.  Keys go from the cache to registers, where every wave expands them for itself; the
+// values' expansion, which has to turn them from tokens to channels, is shared: each wave expands a quarter of the step
+// into LDS (two buffers, one barrier a step), as [8 tokens][channels][16 bytes], the operand as it is read.
+// A row of keys stands for token t(row) with bits 2 and 3 exchanged, so that S^T leaves a lane with eight neighbouring
+// tokens of its query row, which O^T = V^T P^T takes as they are.  Channel j of sixteenth l lies at row 16 j + l of V^T.
+template <int D, int NP>
+struct Rows32 {
+    u4 qf[NP][D / 16];  // query pieces: lane 32 i + n has row n, channels [i D/2, (i+1) D/2)
+    f16v o[D / 32];     // O^T: element e of part k is row 32 k + 8 (e / 4) + 4 i + e % 4 of V^T
+    float m, l;
+};
+
+template <int D>
+struct Keys32 {  // a lane's half of one token's channels
+    u4 k[D / 64];
+    uint32_t ks[D == 256 ? 4 : D == 128 ? 2 : 1];
+};
+
+__device__ __forceinline__ uint32_t token_of_row32(uint32_t r) { return (r & 0x13u) | (r & 4u) << 1 | (r & 8u) >> 1; }
+
+template <int D>
+__device__ __forceinline__ void load_keys32(const uint8_t* p, uint32_t i, uint32_t t, Keys32<D>& x) {
+    constexpr uint32_t QB = D / 8;  // bytes of a quarter of the channels
+#pragma unroll
+    for (uint32_t c = 0; c < D / 64; ++c) {
+        const uint32_t b = c * 16, q = 2 * i + b / QB;
+        if constexpr (D == 64) {  // two quarters, eight bytes each
+            const u2 lo = *(const u2*)(p + (q * 16 + t / 2) * 16 + (t & 1) * 8), hi = *(const u2*)(p + ((q + 1) * 16 + t / 2) * 16 + (t & 1) * 8);
+            x.k[c] = u4{lo[0], lo[1], hi[0], hi[1]};
+        } else {
+            const uint32_t at = (t & 1) * QB + b % QB;
+            x.k[c] = *(const u4*)(p + (at / 16 * 64 + q * 16 + t / 2) * 16);
+        }
+    }
+#pragma unroll
+    for (uint32_t g = 0; g < D / 64; ++g) x.ks[g] = p[16 * D + (i * (D / 64) + g) * 32 + t];
+}
+
+// Rows of 16 bits only: in 32 bits the pieces of 32 rows do not fit the registers.
+template <int D, int T>
+__global__ __launch_bounds__(256, D < 256 ? 2 : 1) void k_kv_attend_rows(KvCache c, KvBatch bt, AttendArgs a) {
+    constexpr int NP = pieces(T), W = D / 16, G = D / 32;
+    __shared__ u4 s_v[2][8 * D];
+    __shared__ uint32_t s_odd[2][4];
+    clear_rest<D, T>(c, bt, a);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t i2 = lane >> 5, n32 = lane & 31u, l16 = lane & 15u, kg = lane >> 4;
+    const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % a.splits;
+    const uint32_t rest = blockIdx.x / c.heads / a.splits, b = rest / a.row_tiles;
+    const uint32_t group = a.q_heads / c.heads, per_page = c.page >> 5;
+    int r0, n;
+    seq_rows(bt, b, r0, n);
+    const int64_t len = max(bt.lengths[b], 0), before = len - n + 1;
+    const int rows = n * (int)group;
+    // the last rows first: with `causal` they have the most to read
+    const int blocks = (rows + 127) / 128;
+    for (int rb = blocks - 1 - (int)(rest % a.row_tiles); rb >= 0; rb -= (int)a.row_tiles) {
+        const int w_first = rb * 128 + (int)wave * 32, row = w_first + (int)n32;
+        const bool live = row < rows;
+        const int64_t limit = !live ? 0 : a.causal ? before + row / (int)group : len;
+        const int64_t most = a.causal ? before + (min(rb * 128 + 127, rows - 1)) / (int)group : len;        // of the workgroup's rows
+        const int64_t w_least = a.causal ? before + w_first / (int)group : len;
+        const uint32_t steps = (tiles_of(c, bt, most) + 1) / 2, chunk = a.chunk / 2;
+        const uint32_t s0 = (uint32_t)min((uint64_t)split * chunk, (uint64_t)steps);
+        const uint32_t s1 = split + 1 == a.splits ? steps : min(s0 + chunk, steps);
+        if (a.splits > 1 && s0 >= s1) continue;  // no part: k_kv_combine does not read it
+        Rows32<D, NP> w;
+        {
+            const uint32_t sign = a.negate ? 0x80000000u : 0u;
+#pragma unroll
+            for (int ch = 0; ch < D / 16; ++ch) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live)
+                    load8<T>(a.q.p, (int64_t)(r0 + row / (int)group) * a.q.row_stride + (int64_t)(h * group + (uint32_t)row % group) * a.q.head_stride +
+                                        i2 * (D / 2) + 8 * ch,
+                             a.q.wide, x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t pc[NP];
+                    pack_pieces<NP>(bits_f32(__float_as_uint(x[2 * e]) ^ sign), bits_f32(__float_as_uint(x[2 * e + 1]) ^ sign), pc);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) w.qf[p][ch][e] = pc[p];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w.o[k][e] = 0.f;
+        w.m = kLowest;
+        w.l = 0.f;
+        Feed<false> feed;
+        auto fill = [&](uint32_t step) {
+            feed.none();
+            if (step + lane / 2 < s1) feed.take(c, bt, b, h, nullptr, 0, (step + lane / 2) * 2 + lane % 2);
+        };
+        Keys32<D> kn[2];
+        u4 vn[D / 64];
+        u2 vsn;
+        bool there_n[2];
+        int32_t base_n = 0;
+        bool v_there_n = false;
+        auto load = [&](uint32_t i) {  // the i-th step of the feed
+            const uint8_t* p[2];
+            const uint32_t ln = opaque(lane);  // addresses are reckoned anew: kept, they would take the registers of the sums
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t lo = __builtin_amdgcn_readlane(feed.lo, 2 * i + x), hi = __builtin_amdgcn_readlane(feed.hi, 2 * i + x);
+                there_n[x] = hi != ~0u;
+                p[x] = c.pool + (there_n[x] ? (uint64_t)hi << 32 | lo : 0) * (uint64_t)(34 * D);
+                load_keys32<D>(p[x], ln >> 5, token_of_row32(ln & 31u), kn[x]);
+            }
+            base_n = (int32_t)__builtin_amdgcn_readlane((uint32_t)feed.pos, 2 * i);
+            const uint8_t* v = wave < 2 ? p[0] : p[1];
+            v_there_n = wave < 2 ? there_n[0] : there_n[1];
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) vn[k] = *(const u4*)(v + 17 * D + (k * 64 + ln) * 16);
+            vsn = *(const u2*)(v + 33 * D + ((ln & 15u) * D / 512) * 32 + 8 * (ln >> 4));
+        };
+        if (s0 < s1) {
+            fill(s0);
+            load(0);
+        }
+        for (uint32_t st = s0; st < s1; ++st) {
+            const uint32_t buf = st & 1u;
+            const int64_t base = base_n;
+            const bool there[2] = {there_n[0], there_n[1]};
+            // this wave's quarter of the values: tile wave / 2, half of each lane's channels
+            {
+                const int64_t seen = v_there_n ? most - base - 32 * (int64_t)(wave >> 1) : 0;
+                u2 vsb = {opaque(vsn[0]), opaque(vsn[1])};
+                uint32_t odd = all_ones_byte(vsb[0]) | all_ones_byte(vsb[1]);
+                if (seen < 32 || __ballot(odd != 0)) {
+                    odd = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t byte = vsb[e / 4] >> (8 * (e % 4)) & 255u;
+                        const bool drop = (int64_t)(8 * kg + e) >= seen;  // seen by no row: it may be anything
+                        if (!drop && byte == 255u) odd = 1;
+                        if (drop || byte == 255u) vsb[e / 4] = (vsb[e / 4] & ~(255u << (8 * (e % 4)))) | 127u << (8 * (e % 4));
+                    }
+                }
+                const uint64_t any = __ballot(odd != 0);
+                if (lane == 0) s_odd[buf][wave] = any != 0;
+                float vs[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vs[e] = bits_f32((vsb[e / 4] >> (8 * (e % 4)) & 255u) << 23);
+                auto expand = [&](auto half) {
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k) {
+                        constexpr int H = decltype(half)::value;
+                        const int jb = H * (D / 64) + k;
+                        u4 even, odd2;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t x = byte_bf16<D / 64>(vn, (2 * r) * (D / 32) + jb, vs[2 * r]);
+                            const uint32_t y = byte_bf16<D / 64>(vn, (2 * r + 1) * (D / 32) + jb, vs[2 * r + 1]);
+                            even[r] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                            odd2[r] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                        }
+                        u4* to = &s_v[buf][((wave >> 1) * 4 + kg) * D + l16];
+                        to[(2 * jb) * 16] = even;
+                        to[(2 * jb + 1) * 16] = odd2;
+                    }
+                };
+                if (wave & 1u) expand(Const<1>());
+                else expand(Const<0>());
+            }
+            f16v s[2];
+            {
+                uint32_t odd = 0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int g = 0; g < D / 64; ++g) kn[x].ks[g] = opaque(kn[x].ks[g]);  // not reckoned with where it is loaded
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[x][e] = 0.f;
+#pragma unroll
+                    for (int ch = 0; ch < D / 16; ++ch) {
+                        const bf8 k8 = as_bf8(codes_bf16(kn[x].k[ch / 4][ch % 4], bits_f32(kn[x].ks[ch / 4] << 23)));
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k8, as_bf8(w.qf[p][ch]), s[x], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int g = 0; g < D / 64; ++g) odd |= kn[x].ks[g] == 255u;
+                    __builtin_amdgcn_sched_barrier(0);  // one tile's keys expanded at a time: their registers are needed
+                }
+                if (base + 64 > w_least || !there[0] || !there[1] || __ballot(odd)) {
+                    const uint32_t i2s = opaque(i2);
+                    const int see = (int)max(min(limit - base, (int64_t)64), (int64_t)0);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        bool bad = false;
+#pragma unroll
+                        for (int g = 0; g < D / 64; ++g) bad |= kn[x].ks[g] == 255u;
+                        uint64_t bb = __ballot(bad);
+                        bb |= bb >> 32;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t r = 8 * (e / 4) + 4 * i2s + e % 4;  // the key's row
+                            if (!there[x] || (bb >> r & 1u)) s[x][e] = __builtin_nanf("");
+                            if ((int)(32 * x + 16 * (e / 8) + 8 * i2s + e % 8) >= see) s[x][e] = -INFINITY;
+                        }
+                    }
+                }
+            }
+            {  // behind the last step: the pool's first tile, not used; without a branch, whose copies would wait for the loads
+                const uint32_t i = (st + 1 - s0) % 32;
+                if (i == 0) fill(st + 1);
+                load(i);
+            }
+            __syncthreads();
+            float top = s[0][0];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
+            {
+                const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(bits_f32(r[0]), bits_f32(r[1])) * a.scale_log2;
+            }
+            const bool over = top > w.m + kSlack;
+            top = over ? top : w.m;
+            if (__ballot(over)) {
+                const float f = __builtin_amdgcn_exp2f(w.m - top);
+                w.m = top;
+                w.l *= f;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) w.o[k][e] *= f;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int ch = 0; ch < 2; ++ch) {
+                    u4 v[D / 32], pf[NP];  // the values are read while the probabilities are reckoned
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) v[k] = s_v[buf][(4 * x + 2 * ch + i2) * D + 32 * k + n32];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * ch + 2 * e], a.scale_log2, -top));
+                        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * ch + 2 * e + 1], a.scale_log2, -top));
+                        uint32_t pc[NP];
+                        pack_pieces<NP>(p0, p1, pc);
+                        w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) pf[p][e] = pc[p];
+                    }
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            w.o[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v[k]), as_bf8(pf[p]), w.o[k], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            if (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3]) {
+                // a value that is not finite: its group's channels of the rows that see it
+                const uint32_t i2s = opaque(i2);
+                for (int t = 0; t < 64; ++t) {
+                    if (!(base + t < limit)) continue;
+                    const int64_t page = page_of(c, bt, b, (uint32_t)((2 * st + t / 32) / per_page));
+                    if (page < 0) continue;
+                    const uint8_t* vs = c.pool + tile_at<D>(c, page, h, (2 * st + t / 32) % per_page) + 33 * D + t % 32;
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t l = 8 * (e / 4 % 2) + 4 * i2s + e % 4;  // sixteenth of the channels
+                            if (vs[(l * W / 32) * 32] == 255u) w.o[k][e] = __builtin_nanf("");
+                        }
+                }
+            }
+        }
+        // each lane has its row's channels [(8 q + 4 i2) W, + 4 W), q = 0, 1
+        {
+            const u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(w.l), __float_as_uint(w.l), false, false);
+            w.l = bits_f32(r[0]) + bits_f32(r[1]);
+        }
+        if (live) {
+            const int token = r0 + row / (int)group;
+            const uint32_t head = h * group + (uint32_t)row % group;
+            const uint64_t at = (uint64_t)token * a.q_heads + head;
+            const float inv = a.splits > 1 ? 1.f : w.l == 0.f ? 0.f : 1.f / w.l;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int c8 = 0; c8 < 4 * W; c8 += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int j = (c8 + e) % W, l4 = (c8 + e) / W;
+                        x[e] = w.o[j / 2][8 * (j % 2) + 4 * q + l4] * inv;
+                    }
+                    const uint32_t d = (8 * q + 4 * i2) * W + c8;
+                    if (a.splits > 1) {
+                        float* po = a.part_o + (at * a.splits + split) * D + d;
+                        *(f4*)po = f4{x[0], x[1], x[2], x[3]};
+                        *(f4*)(po + 4) = f4{x[4], x[5], x[6], x[7]};
+                    } else {
+                        store8<T>(a.out.p, (int64_t)token * a.out.row_stride + (int64_t)head * a.out.head_stride + d, a.out.wide, x);
+                    }
+                }
+            if (i2 == 0) {
+                if (a.splits > 1) *(f2*)(a.part_ml + (at * a.splits + split) * 2) = f2{w.m, w.l};
+                else if (a.lse) a.lse[at] = w.l == 0.f ? -INFINITY : (w.m + __builtin_amdgcn_logf(w.l)) / kLog2e;
+            }
+        }
+        __syncthreads();  // the next rows write the buffers that this one's last step read
+    }
+}
+
 // ---- combine ----------------------------------------------------------------------------
-// A wave joins one row's parts: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 8 lanes hold the channels, the
-// 512 / D groups of them take every so many-th part; the order of the sum is the lanes', alike on every run.
-template <int D, int T, bool CHOSEN>
+// Joins a row's parts: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 8 lanes hold the channels.  FEW (parts of whole
+// rows, at most 16): each of a wave's 512 / D groups of lanes joins a row of its own.  Else the groups share one row and take
+// every so many-th part; the order of the sum is the lanes', alike on every run.
+template <int D, int T, bool CHOSEN, bool FEW>
 __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr uint32_t L = D / 8, G = 64 / L;
     const uint32_t lane = threadIdx.x & 63u, g = lane / L, d = lane % L * 8;
-    const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint64_t wave = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6), at = FEW ? wave * G + g : wave;
     if (at >= (uint64_t)bt.rows * a.q_heads) return;
     const int token = (int)(at / a.q_heads);
     const uint32_t head = at % a.q_heads;
@@ -919,14 +1385,14 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
     seq_rows(bt, b, r0, n);
     uint64_t first, step;  // where the parts lie
     uint32_t parts;
-    if (a.lanes > 0) {
+    if (!FEW && a.lanes > 0) {
         const uint32_t group = a.q_heads / c.heads;
         const uint32_t row = (CHOSEN ? 0u : (uint32_t)(token - r0)) * group + head % group;
         const uint32_t u = (CHOSEN ? (uint32_t)token : b) * a.row_tiles + row / 16;
         const uint32_t p0 = a.prefix[u], p1 = a.prefix[u + 1], total = a.prefix[a.units];
         const uint32_t share = max(a.least / kStep<D, pieces(T)>, (total + a.lanes - 1) / a.lanes);
         const uint32_t w0 = p0 / share, w1 = p1 > p0 ? (p1 - 1) / share : w0;
-        if (p1 > p0 && w0 == w1) return;  // one workgroup took it whole
+        if (p1 > p0 && w0 == w1) return;  // one wave took it whole
         parts = p1 > p0 ? w1 - w0 + 1 : 0;
         step = a.slot_rows;
         first = ((uint64_t)(head / group) * (a.lanes + a.units) + w0 + u) * a.slot_rows + row % 16;
@@ -939,12 +1405,16 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
         first = at * a.splits;
     }
     float m = kLowest;
-    for (uint32_t s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[(first + s * step) * 2]);
+    if constexpr (FEW) {
+        for (uint32_t s = 0; s < parts; ++s) m = fmaxf(m, a.part_ml[(first + s) * 2]);
+    } else {
+        for (uint32_t s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[(first + s * step) * 2]);
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+        for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    }
     float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (uint32_t s = g; s < parts; s += G) {
+    for (uint32_t s = FEW ? 0 : g; s < parts; s += FEW ? 1 : G) {
         const uint64_t p = first + s * step;
         const f2 ml = *(const f2*)(a.part_ml + p * 2);
         const float* po = a.part_o + p * D + d;
@@ -954,13 +1424,15 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += u[i] * f, o[4 + i] += v[i] * f;
     }
+    if constexpr (!FEW) {
 #pragma unroll
-    for (uint32_t x = L; x < 64; x <<= 1) {
-        l += __shfl_xor(l, (int)x);
+        for (uint32_t x = L; x < 64; x <<= 1) {
+            l += __shfl_xor(l, (int)x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] += __shfl_xor(o[i], (int)x);
+            for (int i = 0; i < 8; ++i) o[i] += __shfl_xor(o[i], (int)x);
+        }
+        if (g) return;
     }
-    if (g) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] *= inv;
@@ -972,153 +1444,356 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
 // Score of a page for a query head: 2^(a + b) * sum_d max(q8_d, 0) hi_d + min(q8_d, 0) lo_d with q8 = rint(q / 2^a) and the
 // page's bounds hi, lo in units of 2^b.  The sum is a product of whole numbers over 2 D channels: v_mfma_i32_16x16x64_i8,
 // exact in any order.  A wave scores 16 pages for 16 columns: `width` columns (a power of two) a token, the group's heads.
-template <int D, int T>
-__global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t chunks) {
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
-    const uint32_t h = blockIdx.x % c.heads, chunk = blockIdx.x / c.heads % chunks;
-    const uint32_t unit = blockIdx.x / c.heads / chunks;
-    const uint32_t b = unit / tok_tiles;
-    int r0, n;
-    seq_rows(bt, b, r0, n);
-    const int64_t len = max(bt.lengths[b], 0);
-    const uint32_t group = a.q_heads / c.heads;
-    const uint32_t width = min(16u, next_pow2(group)), per = 16 / width;
-    for (int tt = (int)(unit % tok_tiles); tt * (int)per < n; tt += (int)tok_tiles) {
-        const int tok = tt * (int)per + (int)(n16 / width);
-        const bool live = tok < n;
-        const int last = min(tt * (int)per + (int)per, n) - 1;
-        const int64_t seen = min(a.pages_seen(c, bt, a.causal ? len - n + last + 1 : len), (int64_t)bt.table_width);
-        if ((int64_t)chunk * a.score_chunk >= seen) continue;
-        const int64_t p_end = chunk + 1 == chunks ? seen : min(seen, ((int64_t)chunk + 1) * a.score_chunk);
-        for (int64_t p0 = (int64_t)chunk * a.score_chunk + wave * 16; p0 < p_end; p0 += 64) {
-            const int64_t pm = p0 + n16;
-            const int64_t page = pm < seen ? page_of(c, bt, b, (uint32_t)pm) : -1;
-            u4 bd[D / 32];
-            uint32_t e = 255u;
-            const int8_t* row = c.bounds + ((uint64_t)max(page, (int64_t)0) * c.heads + h) * (2 * D);
+template <int D>
+struct ScoreCols {  // this lane's column: channels k * 64 + q4 * 16 .. + 16 in 8 bits
+    u4 pos[D / 64], neg[D / 64];
+    uint32_t e;  // biased exponent of the column's largest magnitude
+    bool on;
+
+    template <int T>
+    __device__ __forceinline__ void load(const AttendArgs& a, bool live, int64_t at, uint32_t q4) {
+        on = live;
+        float x[D / 64][16];
+        uint32_t amax = 0;
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) bd[k] = *(const u4*)(row + k * 64 + q4 * 16);
-            if (page >= 0) e = c.bound_exps[(uint64_t)page * c.heads + h];
-            float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            for (uint32_t g0 = 0; g0 < group; g0 += width) {
-                const uint32_t gh = g0 + n16 % width;
-                const bool on = live && gh < group;
-                float x[D / 64][16];
-                uint32_t amax = 0;
+        for (int k = 0; k < D / 64; ++k)
 #pragma unroll
-                for (int k = 0; k < D / 64; ++k)
+            for (int half = 0; half < 2; ++half) {
+                float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (on) load8<T>(a.q.p, at + k * 64 + q4 * 16 + half * 8, a.q.wide, y);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                        if (on)
-                            load8<T>(a.q.p, (int64_t)(r0 + tok) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride + k * 64 + q4 * 16 + half * 8,
-                                     a.q.wide, y);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            x[k][half * 8 + i] = y[i];
-                            amax = max(amax, __float_as_uint(y[i]) & 0x7FFFFFFFu);
-                        }
-                    }
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-                const uint32_t qe = min(max((amax + 0x1FFFFu) >> 23, 7u), 255u);
-                const float up = amax >= 0x7F800000u ? 0.f : bits_f32((260u - qe) << 23);
-                i4 acc = {0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < D / 64; ++k) {
-                    u4 pos, neg;
-#pragma unroll
-                    for (int wd = 0; wd < 4; ++wd) {
-                        uint32_t pp = 0, nn = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int v = amax >= 0x7F800000u ? 0 : (int)rintf(x[k][wd * 4 + i] * up);
-                            pp |= (uint32_t)(max(v, 0) & 255) << (8 * i);
-                            nn |= (uint32_t)(min(v, 0) & 255) << (8 * i);
-                        }
-                        pos[wd] = pp, neg[wd] = nn;
-                    }
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, bd[k]), __builtin_bit_cast(i4, pos), acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, bd[D / 64 + k]), __builtin_bit_cast(i4, neg), acc, 0, 0, 0);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t be = (uint32_t)__shfl((int)e, 4 * (int)q4 + r);
-                    const int ex = min(max((int)qe + (int)be - 266, -126), 127);
-                    float sc = on ? (float)acc[r] * bits_f32((uint32_t)(ex + 127) << 23) : -INFINITY;
-                    for (uint32_t x2 = 1; x2 < width; x2 <<= 1) sc = fmaxf(sc, __shfl_xor(sc, (int)x2));
-                    best[r] = be == 255u ? 3.402823466e38f : fmaxf(best[r], sc);
+                for (int i = 0; i < 8; ++i) {
+                    x[k][half * 8 + i] = y[i];
+                    amax = max(amax, __float_as_uint(y[i]) & 0x7FFFFFFFu);
                 }
             }
-            if (live && n16 % width == 0) {
-                float* out = a.scores + ((uint64_t)(r0 + tok) * c.heads + h) * bt.table_width + p0 + 4 * q4;
+        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+        e = min(max((amax + 0x1FFFFu) >> 23, 7u), 255u);
+        const bool finite = amax < 0x7F800000u;  // else every score is 0
+        const float up = bits_f32((260u - e) << 23);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (p0 + 4 * q4 + r < seen) out[r] = best[r];
+        for (int k = 0; k < D / 64; ++k)
+#pragma unroll
+            for (int wd = 0; wd < 4; ++wd) {
+                uint32_t pp = 0, nn = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int v = finite ? (int)rintf(x[k][wd * 4 + i] * up) : 0;
+                    pp |= (uint32_t)(max(v, 0) & 255) << (8 * i);
+                    nn |= (uint32_t)(min(v, 0) & 255) << (8 * i);
+                }
+                pos[k][wd] = pp, neg[k][wd] = nn;
+            }
+    }
+};
+
+// Each lane's values and those of the lane that a DPP control names (quad_perm exchanges of 1 and 2, half and whole row mirrors:
+// after the exchanges below them they reach every lane of 4, 8 and 16).
+template <int CTRL>
+__device__ __forceinline__ void row_max_step(float (&v)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int x = (int)__float_as_uint(v[r]);
+        v[r] = fmaxf(v[r], __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false)));
+    }
+}
+
+// best[r]: the largest score over the columns of this lane's token, of page 4 q4 + r of 16.  Lane 16 q + m holds page m's channels
+// q * 16 .. + 16 of every 64 in pb; lane first + m its exponent in e (255: not finite, or not there).
+template <int D>
+__device__ __forceinline__ void score_pages(const u4 (&pb)[D / 32], uint32_t e, uint32_t first, const ScoreCols<D>& col, uint32_t width,
+                                            uint32_t q4, float (&best)[4]) {
+    i4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, pb[k]), __builtin_bit_cast(i4, col.pos[k]), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, pb[D / 64 + k]), __builtin_bit_cast(i4, col.neg[k]), acc, 0, 0, 0);
+    }
+    uint32_t be[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) be[r] = (uint32_t)__shfl((int)e, (int)(first + 4 * q4) + r);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int ex = min(max((int)col.e + (int)be[r] - 266, -126), 127);
+        best[r] = col.on ? (float)acc[r] * bits_f32((uint32_t)(ex + 127) << 23) : -INFINITY;
+    }
+    // over the token's columns: pairs, fours, eights, all 16 lanes of a row
+    if (width > 1) row_max_step<0xB1>(best);
+    if (width > 2) row_max_step<0x4E>(best);
+    if (width > 4) row_max_step<0x141>(best);
+    if (width > 8) row_max_step<0x140>(best);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) best[r] = be[r] == 255u ? 3.402823466e38f : best[r];
+}
+
+// Scores of pages [from, to) for 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256: half
+// of them); `put` takes four neighbouring pages' scores.
+template <int D, class Put>
+__device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt, uint32_t b, uint32_t h, const ScoreCols<D>& col, uint32_t width,
+                                            int64_t from, int64_t to, uint32_t wave, uint32_t waves, uint32_t lane, Put put) {
+    constexpr int NB = D == 256 ? 2 : 4;
+    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
+    auto look = [&](int64_t p) { return p + lane < to ? (int)page_of(c, bt, b, (uint32_t)(p + lane)) : -1; };
+    int64_t p = from + wave * 64;
+    int page = p < to ? look(p) : -1;
+    for (; p < to; p += waves * 64) {
+        const uint32_t e = page >= 0 ? c.bound_exps[(uint64_t)page * c.heads + h] : 255u;
+        const int now = page;
+#pragma unroll
+        for (int s = 0; s < 4; s += NB) {
+            if (p + 16 * s >= to) break;
+            u4 pb[NB][D / 32];
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
+                const int pg = max(__shfl(now, (int)(16 * (s + x) + n16)), 0);  // one that is not there: its exponent says so
+                const int8_t* row = c.bounds + ((uint64_t)pg * c.heads + h) * (2 * D) + q4 * 16;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) pb[x][k] = *(const u4*)(row + k * 64);
+            }
+            if (s + NB == 4) page = look(p + waves * 64);
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
+                float best[4];
+                score_pages<D>(pb[x], e, 16 * (s + x), col, width, q4, best);
+                put(p + 16 * (s + x) + 4 * q4, best);
             }
         }
     }
 }
 
-// The `top` pages of one token and key head: the first and the most recent ones, then the largest scores, the
-// lowest page among equals; written in order, -1 behind the last.  Four passes over the scores find the
-// top-th largest key eight bits at a time.
-__global__ __launch_bounds__(256) void k_kv_select(KvCache c, KvBatch bt, AttendArgs a) {
-    __shared__ uint32_t hist[256], wsum[4], s_digit, s_above;
+// ---- choosing ------------------------------------------------------------------------------
+// The `top` of a token's `seen` pages (more than `top`): the first and the most recent ones, then the largest scores, the lowest
+// page among equals; in order.
+//
+// The want-th largest of the lanes' own maxima is no more than the want-th largest of all keys: what is below it is dropped at
+// once, and a list little longer than `want` is left.  On it the interval of keys that holds the last one taken is halved until
+// it parts the list; one wave, no barrier.  Code that runs once is slow to fetch: the loops are kept rolled.
+constexpr uint32_t kListWave = 256;   // list entries a wave
+constexpr uint32_t kChooseThreads = 512, kChooseWaves = kChooseThreads / 64;
+struct ChooseLds {
+    uint32_t key[kChooseWaves * kListWave], page[kChooseWaves * kListWave];
+    uint32_t most[kChooseThreads], count[kChooseWaves];
+};
+
+// The interval [lo, hi): `want` or more of the n keys are >= lo, fewer (`over`) are >= hi.  true: from `want` to `want` + `slack` are
+// >= lo; false: [lo, hi) is one key.
+template <class Key>
+__device__ __forceinline__ bool halve(Key key, uint32_t n, uint32_t want, uint32_t slack, uint32_t& lo, uint32_t hi, uint32_t& over,
+                                      uint32_t lane) {
+    constexpr int K = 8;  // keys a lane: the list, or the lanes' maxima
+    over = 0;
+    uint32_t k[K];
+    const bool few = n <= 64 * K;
+#pragma unroll
+    for (int i = 0; i < K; ++i) k[i] = few && lane + 64 * i < n ? key(lane + 64 * i) : 0;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        uint32_t c = 0;
+        if (few) {
+#pragma unroll
+            for (int i = 0; i < K; ++i) c += (uint32_t)__popcll(__ballot(k[i] >= mid));
+        } else {
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; i += 64) c += (uint32_t)__popcll(__ballot(i + lane < n && key(min(i + lane, n - 1)) >= mid));
+        }
+        if (c >= want) lo = mid;
+        else hi = mid, over = c;
+        if (c >= want && c - want <= slack) return true;
+    }
+    return false;
+}
+
+// W waves together (`wave` of them; barriers where W > 1), or one wave by itself.
+template <uint32_t W, class Scores>
+__device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uint32_t seen, int32_t* out, ChooseLds& s, uint32_t wave,
+                                             uint32_t lane) {
+    auto meet = [] {
+        if constexpr (W > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    const uint32_t part = W > 1 ? wave : 0, home = W > 1 ? 0 : wave;  // of the pages, and where the list begins
+    const uint32_t lo_j = a.first, hi_j = seen - a.recent, want = a.top - a.first - a.recent;
+    const uint32_t each = ((hi_j - lo_j + W - 1) / W + 63) / 64 * 64;  // a wave's pages, side by side: the list is in order
+    const uint32_t j0 = min(lo_j + part * each, hi_j), j1 = min(j0 + each, hi_j);
+    uint32_t* const list_key = s.key + home * kListWave;
+    uint32_t* const list_page = s.page + home * kListWave;
+    constexpr uint32_t kCap = kListWave * W;
+    // the lanes' maxima, and the least and largest of them
+    uint32_t most = 0;
+#pragma unroll 4
+    for (uint32_t j = j0 + lane; j < j1; j += 64) most = max(most, f32_order(sc(j)));
+    s.most[wave * 64 + lane] = most;
+    meet();
+    uint32_t hi = 0, floor = 0;
+    auto maxima = [&](uint32_t i) { return s.most[(W > 1 ? 0 : wave * 64) + i]; };
+#pragma unroll 1
+    for (uint32_t i = lane; i < W * 64; i += 64) hi = max(hi, maxima(i));
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, x));
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    uint32_t over;
+    if (want > 0 && want <= W * 64) (void)halve(maxima, W * 64, want, 2 * W, floor, hi + 1, over, lane);
+    // the list of what is left; where it is too long, the pages themselves are gone over
+    uint32_t mine = 0;
+#pragma unroll 2
+    for (uint32_t j = j0; j < j1; j += 64) mine += (uint32_t)__popcll(__ballot(j + lane < j1 && f32_order(sc(min(j + lane, j1 - 1))) >= floor));
+    if (lane == 0) s.count[wave] = mine;
+    meet();
+    uint32_t at = 0, n = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+        const uint32_t x = s.count[W > 1 ? w : wave];
+        if (w < part) at += x;
+        n += x;
+    }
+    const bool listed = n <= kCap;
+    if (listed) {
+#pragma unroll 1
+        for (uint32_t j = j0; j < j1; j += 64) {
+            const uint32_t k = j + lane < j1 ? f32_order(sc(j + lane)) : 0u;
+            const bool in = j + lane < j1 && k >= floor;
+            const uint64_t m = __ballot(in);
+            const uint32_t to = at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
+            if (in) list_key[to] = k, list_page[to] = j + lane;
+            at += (uint32_t)__popcll(m);
+        }
+    }
+    meet();
+    if (W == 1 || wave == 0) {
+        for (uint32_t i = lane; i < a.first; i += 64) out[i] = (int32_t)i;
+        for (uint32_t i = lane; i < a.recent; i += 64) out[a.first + want + i] = (int32_t)(hi_j + i);
+        if (want > 0) {
+            if (!listed) n = hi_j - lo_j, floor = 0;
+            auto key = [&](uint32_t i) { return listed ? list_key[i] : f32_order(sc(lo_j + i)); };
+            uint32_t lo = floor;
+            const bool exact = n > want && halve(key, n, want, 0, lo, hi + 1, over, lane);
+            // n == want: all; else those over lo, and the first `ties` that equal it
+            const uint32_t ties = n == want ? ~0u : exact ? ~0u : want - over;
+            uint32_t put = a.first, tied = 0;
+#pragma unroll 1
+            for (uint32_t i = 0; i < n; i += 64) {
+                const uint32_t k = i + lane < n ? key(i + lane) : 0u;
+                const bool same = i + lane < n && k == lo;
+                const uint64_t sm = __ballot(same), below = (1ull << lane) - 1ull;
+                const bool take = (i + lane < n && k > lo) || (same && tied + (uint32_t)__popcll(sm & below) < ties);
+                const uint64_t tm = __ballot(take);
+                if (take) out[put + (uint32_t)__popcll(tm & below)] = (int32_t)(listed ? list_page[i + lane] : lo_j + i + lane);
+                put += (uint32_t)__popcll(tm);
+                tied += (uint32_t)__popcll(sm);
+            }
+        }
+    }
+    meet();
+}
+
+// One workgroup: the pages of 16 / width tokens of a sequence (`per` of them here) and one key head, scored into LDS and chosen
+// there.  Bound by the bounds that it reads, 2 D + 1 bytes a page.
+template <int D, int T>
+__global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t per) {
+    extern __shared__ float s_sc[];  // [per][table_width]
+    __shared__ ChooseLds s_choose;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
+    const uint32_t h = blockIdx.x % c.heads, unit = blockIdx.x / c.heads, b = unit / tok_tiles;
+    int r0, n;
+    seq_rows(bt, b, r0, n);
+    const int64_t before = (int64_t)max(bt.lengths[b], 0) - n + 1;
+    const uint32_t group = a.q_heads / c.heads, width = min(16u, next_pow2(group));
+    for (int t0 = (int)(unit % tok_tiles) * (int)per; t0 < n; t0 += (int)(tok_tiles * per)) {
+        const int toks = min((int)per, n - t0);
+        const int64_t have = a.pages_seen(c, bt, before + t0 + toks - 1), seen = min(have, (int64_t)bt.table_width);
+        if (have > (int64_t)a.top) {
+            const uint32_t my = n16 / width;  // this lane's token of the tile
+            for (uint32_t g0 = 0; g0 < group; g0 += width) {
+                const uint32_t gh = g0 + n16 % width;
+                ScoreCols<D> col;
+                col.template load<T>(a, (int)my < toks && gh < group,
+                                     (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+                score_range<D>(c, bt, b, h, col, width, 0, seen, wave, kChooseThreads / 64, lane, [&](int64_t p, const float(&best)[4]) {
+                    if ((int)my >= toks || n16 % width) return;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (p + r < seen) {
+                            float* to = &s_sc[my * bt.table_width + p + r];
+                            *to = g0 ? fmaxf(*to, best[r]) : best[r];
+                        }
+                });
+            }
+        }
+        __syncthreads();
+        const uint32_t in_lds = bt.table_width;
+        for (int t = 0; t < toks; ++t) {
+            const int64_t mine = a.pages_seen(c, bt, before + t0 + t);
+            int32_t* out = a.chosen + ((uint64_t)(r0 + t0 + t) * c.heads + h) * a.top;
+            const float* sc = s_sc + t * bt.table_width;
+            // a page beyond the table is the last: it is among the recent ones, or scores as one that is not there
+            auto score = [=](uint32_t j) { return j < in_lds ? sc[j] : 3.402823466e38f; };
+            if (mine > (int64_t)a.top && toks == 1) {
+                choose_pages<kChooseWaves>(a, score, (uint32_t)mine, out, s_choose, wave, lane);
+            } else if ((uint32_t)t % kChooseWaves == wave) {  // each wave its token
+                if (mine > (int64_t)a.top) {
+                    choose_pages<1>(a, score, (uint32_t)mine, out, s_choose, wave, lane);
+                } else {
+                    for (uint32_t i = lane; i < a.top; i += 64) out[i] = (int64_t)i < mine ? (int32_t)i : -1;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds.
+template <int D, int T>
+__global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t chunks) {
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t q4 = lane >> 4, n16 = lane & 15u;
+    const uint32_t h = blockIdx.x % c.heads, chunk = blockIdx.x / c.heads % chunks;
+    const uint32_t unit = blockIdx.x / c.heads / chunks, b = unit / tok_tiles;
+    int r0, n;
+    seq_rows(bt, b, r0, n);
+    const int64_t before = (int64_t)max(bt.lengths[b], 0) - n + 1;
+    const uint32_t group = a.q_heads / c.heads, width = min(16u, next_pow2(group)), per = 16 / width;
+    for (int t0 = (int)(unit % tok_tiles) * (int)per; t0 < n; t0 += (int)(tok_tiles * per)) {
+        const int toks = min((int)per, n - t0);
+        const int64_t seen = min(a.pages_seen(c, bt, before + t0 + toks - 1), (int64_t)bt.table_width);
+        const int64_t from = (int64_t)chunk * a.score_chunk;
+        const int64_t to = chunk + 1 == chunks ? seen : min(seen, from + (int64_t)a.score_chunk);
+        const uint32_t my = n16 / width;
+        for (uint32_t g0 = 0; g0 < group && from < to; g0 += width) {
+            const uint32_t gh = g0 + n16 % width;
+            ScoreCols<D> col;
+            col.template load<T>(a, (int)my < toks && gh < group,
+                                 (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+            score_range<D>(c, bt, b, h, col, width, from, to, wave, 4, lane, [&](int64_t p, const float(&best)[4]) {
+                if ((int)my >= toks || n16 % width) return;
+                float* out = a.scores + ((uint64_t)(r0 + t0 + (int)my) * c.heads + h) * bt.table_width + p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (p + r < to) out[r] = g0 ? fmaxf(out[r], best[r]) : best[r];
+            });
+        }
+    }
+}
+
+__global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch bt, AttendArgs a) {
+    __shared__ ChooseLds s_choose;
     const uint32_t h = blockIdx.x % c.heads;
     const int token = (int)(blockIdx.x / c.heads);
     uint32_t b;
     if (!a.row_seq(bt, token, b)) return;
     int r0, n;
     seq_rows(bt, b, r0, n);
-    const int64_t len = max(bt.lengths[b], 0);
-    const int64_t seen = a.pages_seen(c, bt, a.causal ? len - n + (token - r0) + 1 : len);
+    const int64_t seen = a.pages_seen(c, bt, (int64_t)max(bt.lengths[b], 0) - n + (token - r0) + 1);
     int32_t* out = a.chosen + ((uint64_t)token * c.heads + h) * a.top;
     if (seen <= (int64_t)a.top) {
-        for (uint32_t i = threadIdx.x; i < a.top; i += 256) out[i] = (int64_t)i < seen ? (int32_t)i : -1;
+        for (uint32_t i = threadIdx.x; i < a.top; i += kChooseThreads) out[i] = (int64_t)i < seen ? (int32_t)i : -1;
         return;
     }
     const float* sc = a.scores + ((uint64_t)token * c.heads + h) * bt.table_width;
-    auto key = [&](uint32_t j) -> uint32_t {
-        if (j < a.first || (int64_t)j >= seen - (int64_t)a.recent || j >= bt.table_width) return 0xFFFFFFFFu;
-        return f32_order(sc[j]);
-    };
-    const uint32_t N = (uint32_t)seen;
-    uint32_t prefix = 0, mask = 0, want = a.top;  // the want-th largest among keys with this prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t j = threadIdx.x; j < N; j += 256) {
-            const uint32_t k = key(j);
-            if ((k & mask) == prefix) atomicAdd(&hist[255u - (k >> shift & 255u)], 1u);  // LDS counts: any order
-        }
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const uint32_t t = wave_find_cum(hist, 256, want);
-            const uint32_t above = wave_sum_below(hist, t);
-            if (threadIdx.x == 0) s_digit = 255u - t, s_above = above;
-        }
-        __syncthreads();
-        prefix |= s_digit << shift;
-        mask |= 255u << shift;
-        want -= s_above;
-        __syncthreads();
-    }
-    // keys over the found one, and the first `want` that equal it, in page order
-    uint32_t put = 0, ties = 0;
-    for (uint32_t j0 = 0; j0 < N; j0 += 256) {
-        const uint32_t j = j0 + threadIdx.x;
-        const uint32_t k = j < N ? key(j) : 0u;
-        const bool over = j < N && k > prefix, same = j < N && k == prefix;
-        uint32_t tot_same, tot;
-        const uint32_t before = big_prefix(same, wsum, &tot_same);
-        const bool take = over || (same && ties + before < want);
-        const uint32_t at = big_prefix(take, wsum, &tot);
-        if (take && put + at < a.top) out[put + at] = (int32_t)j;
-        put += tot;
-        ties += tot_same;
-    }
+    const uint32_t width = bt.table_width;
+    choose_pages<kChooseWaves>(a, [=](uint32_t j) { return j < width ? sc[j] : 3.402823466e38f; }, (uint32_t)seen, out, s_choose,
+                               __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63u);
 }
 
 }  // namespace
@@ -1134,6 +1809,15 @@ __global__ __launch_bounds__(256) void k_kv_select(KvCache c, KvBatch bt, Attend
         case GVDB_F32: KV_DT(D_, GVDB_F32, body) break;        \
         case GVDB_F16: KV_DT(D_, GVDB_F16, body) break;        \
         default: KV_DT(D_, GVDB_BF16, body) break;             \
+    }
+#define KV_T16(D_, dtype, body)                                \
+    if ((dtype) == GVDB_F16) KV_DT(D_, GVDB_F16, body)         \
+    else KV_DT(D_, GVDB_BF16, body)
+#define KV_DISPATCH16(dim, dtype, body)          \
+    switch (dim) {                               \
+        case 64: KV_T16(64, dtype, body) break;   \
+        case 128: KV_T16(128, dtype, body) break; \
+        default: KV_T16(256, dtype, body) break;  \
     }
 #define KV_DISPATCH(dim, dtype, body)            \
     switch (dim) {                               \
@@ -1161,7 +1845,8 @@ hipError_t launch_kv_append(const KvCache& c, const KvBatch& bt, const KvRows& k
 }
 
 hipError_t launch_kv_read(const KvCache& c, const KvBatch& bt, const KvRows& k, const KvRows& v, hipStream_t s) {
-    const uint64_t blocks = ((uint64_t)bt.rows * c.heads * (c.dim / 8) + 255) / 256;
+    const uint32_t tokens = 256 / (c.dim / 8);  // a workgroup
+    const uint64_t blocks = ((uint64_t)bt.rows + tokens - 1) / tokens * c.heads;
     if (!fits(blocks)) return hipErrorInvalidValue;
     const uint32_t dtype = k.p ? k.dtype : v.dtype;
     KV_DISPATCH(c.dim, dtype, (k_kv_read<D, T><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, k, v)));
@@ -1171,16 +1856,23 @@ hipError_t launch_kv_read(const KvCache& c, const KvBatch& bt, const KvRows& k, 
 
 hipError_t launch_kv_attend(const KvCache& c, const KvBatch& bt, const AttendArgs& a, hipStream_t s) {
     const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.n_seqs);
-    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + 3) / 4;
+    const bool few = !a.lanes && a.splits <= 16;
+    const uint64_t per_join = few ? 4 * (512 / c.dim) : 4, joins = ((uint64_t)bt.rows * a.q_heads + per_join - 1) / per_join;
     if (!fits(blocks) || !fits(joins)) return hipErrorInvalidValue;
     if (a.lanes) {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend_line<D, T, false><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
+    } else if (a.many) {
+        KV_DISPATCH16(c.dim, a.q.dtype, (k_kv_attend_rows<D, T><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
     } else {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, false><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
     }
     GVDB_LAUNCH_CHECK();
     if (a.lanes || a.splits > 1) {
-        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, false><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        if (few) {
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, false, true><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        } else {
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, false, false><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        }
         GVDB_LAUNCH_CHECK();
     }
     return hipSuccess;
@@ -1188,17 +1880,28 @@ hipError_t launch_kv_attend(const KvCache& c, const KvBatch& bt, const AttendArg
 
 hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const AttendArgs& a, hipStream_t s) {
     const uint32_t group = a.q_heads / c.heads;
-    const uint32_t per = 16 / (group >= 16 ? 16 : next_pow2(group));
-    const uint32_t chunks = (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
+    uint32_t per = 16 / (group >= 16 ? 16 : next_pow2(group));
+    if (bt.max_new < per) per = next_pow2(bt.max_new);
+    const bool fused = a.score_chunk == 0;
+    while (fused && per > 1 && per * bt.table_width > kChooseScores) per /= 2;
+    const uint32_t chunks = fused ? 1 : (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
     const uint64_t others = (uint64_t)c.heads * chunks * bt.n_seqs;
     const uint32_t tok_tiles = capped(((uint64_t)bt.max_new + per - 1) / per, others, 1u << 22);
     const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.rows);
-    const uint64_t joins = ((uint64_t)bt.rows * a.q_heads + 3) / 4;
+    const bool few = !a.lanes && a.splits <= 16;
+    const uint64_t per_join = few ? 4 * (512 / c.dim) : 4, joins = ((uint64_t)bt.rows * a.q_heads + per_join - 1) / per_join;
     if (!fits(others * tok_tiles) || !fits(blocks) || !fits(joins) || !fits((uint64_t)bt.rows * c.heads)) return hipErrorInvalidValue;
-    KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));
-    GVDB_LAUNCH_CHECK();
-    k_kv_select<<<bt.rows * c.heads, 256, 0, s>>>(c, bt, a);
-    GVDB_LAUNCH_CHECK();
+    if (fused) {
+        const uint32_t lds = per * bt.table_width * 4;
+        KV_DISPATCH(c.dim, a.q.dtype,
+                    (k_kv_choose<D, T><<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
+        GVDB_LAUNCH_CHECK();
+    } else {
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));
+        GVDB_LAUNCH_CHECK();
+        k_kv_select<<<bt.rows * c.heads, kChooseThreads, 0, s>>>(c, bt, a);
+        GVDB_LAUNCH_CHECK();
+    }
     if (a.lanes) {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend_line<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
     } else {
@@ -1206,7 +1909,11 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
     }
     GVDB_LAUNCH_CHECK();
     if (a.lanes || a.splits > 1) {
-        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        if (few) {
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true, true><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        } else {
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true, false><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
+        }
         GVDB_LAUNCH_CHECK();
     }
     return hipSuccess;

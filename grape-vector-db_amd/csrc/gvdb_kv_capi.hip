@@ -92,7 +92,8 @@ gvdb_status take_rows(const gvdb_kv_rows* in, const char* what, KvRows& r) {
     if (in->dtype > GVDB_BF16) return invalid((std::string("token cache: unknown dtype of ") + what).c_str());
     const uint32_t size = size_of(in->dtype);
     if ((uintptr_t)in->data % size) return invalid((std::string("token cache: misaligned ") + what).c_str());
-    r = {in->data, in->dtype, in->row_stride, in->head_stride, false};
+    if (in->flags > GVDB_KV_ZERO_REST) return invalid((std::string("token cache: unknown flags of ") + what).c_str());
+    r = {in->data, in->dtype, in->row_stride, in->head_stride, false, in->flags == GVDB_KV_ZERO_REST};
     r.wide = ((uint64_t)(uintptr_t)in->data | (uint64_t)in->row_stride * size | (uint64_t)in->head_stride * size) % 16 == 0;
     return GVDB_OK;
 }
@@ -105,7 +106,7 @@ struct Plan {
     uint64_t scores = 0, chosen = 0, part_o = 0, part_ml = 0, prefix = 0, bytes = 0;
 };
 
-gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t q_heads, uint32_t top, Plan& p) {
+gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uint32_t q_heads, uint32_t top, Plan& p) {
     if (q_heads == 0 || q_heads % c.heads || q_heads > 65536)
         return invalid("token cache: q_heads is a multiple of kv_heads, at most 65536");
     if (top > 65536) return invalid("token cache: top is at most 65536");
@@ -116,20 +117,25 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t q_heads, u
     const uint64_t tiles = top ? (uint64_t)std::min(top, bt.table_width) * (c.page / 32) : ((uint64_t)bt.max_len + 31) / 32;
     const uint64_t rows_each = top ? group : bt.max_new * group;
     const uint64_t units0 = top ? bt.rows : bt.n_seqs;
-    uint64_t row_tiles = (rows_each + 15) / 16;
+    // 128 rows and more share the values' expansion: a chunk of 2048 tokens takes 632 us so and 1110 us in tiles of 16 rows; at 64 rows
+    // a sequence 40 and 35 us, at 128 rows 49 and 50.  In 32 bits the pieces do not fit the registers: 130 and 117 us at 512 rows.
+    a.many = !top && dtype != GVDB_F32 && rows_each >= 128;
+    uint64_t row_tiles = a.many ? (rows_each + 127) / 128 : (rows_each + 15) / 16;
     // grids stay below 2^20 tiles of rows where the hints are loose: the kernels stride over the rest
     row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
     const uint64_t units = units0 * c.heads * row_tiles;
+    // workgroups that have rows: with `cu` the sequences are of several lengths, and `rows` says how many there are in all
+    const uint64_t busy = top ? units : std::min(units, (bt.rows * group / (a.many ? 128 : 16) + bt.n_seqs) * c.heads);
     // Two workgroups a CU: four waves a SIMD pair read 5.3 TB/s.  64 sequences of up to 10000 tokens: 65 us with one, 58 with
     // two, 69 with three, 65 with four; 4 x 256K tokens: 263, 215, 231, 226 us.
     const uint64_t slots = 512;
     a.row_tiles = (uint32_t)row_tiles;
     a.splits = 1;
     a.chunk = (uint32_t)(tiles + 1) / 2 * 2;
-    if (tiles > 32 && units < 4 * slots) {  // else a workgroup takes its rows' tiles whole
+    if (a.many ? busy < 2 * slots && tiles > 32 : tiles > 32 && units < 4 * slots) {  // else a workgroup takes its rows' tiles whole
         const uint64_t line = units0 * ((rows_each + 15) / 16);
         const uint64_t most = line * (top ? (uint64_t)top : (uint64_t)bt.table_width + 1) * (c.page / 32);
-        if ((top || !bt.cu) && line <= kMaxUnits && most < (1ull << 31)) {
+        if (!a.many && (top || !bt.cu) && line <= kMaxUnits && most < (1ull << 31)) {
             // the rows of a unit are known: every wave gets the same share of all tiles, of 4 at least
             a.units = (uint32_t)line;
             a.lanes = (uint32_t)std::max<uint64_t>(1, slots / c.heads) * 4;
@@ -137,7 +143,7 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t q_heads, u
             a.slot_rows = (uint32_t)std::min<uint64_t>(16, rows_each);
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
         } else {
-            a.chunk = (uint32_t)std::max<uint64_t>(8, ((units * tiles + slots - 1) / slots + 1) / 2 * 2);  // whole steps
+            a.chunk = (uint32_t)std::max<uint64_t>(a.many ? 16 : 8, ((busy * tiles + 2 * slots - 1) / (2 * slots) + 1) / 2 * 2);  // whole steps
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         }
     }
@@ -145,9 +151,12 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t q_heads, u
     const uint64_t qr = (uint64_t)bt.rows * q_heads;
     uint64_t at = 0;
     if (top) {
-        a.score_chunk = 256;
-        p.scores = at;
-        at += up256((uint64_t)bt.rows * c.heads * bt.table_width * 4);
+        const bool split = bt.table_width > kChooseScores || (kv_max_pages(c, bt) > 512 && (uint64_t)bt.rows * c.heads <= 1024);
+        a.score_chunk = split ? 256 : 0;
+        if (split) {
+            p.scores = at;
+            at += up256((uint64_t)bt.rows * c.heads * bt.table_width * 4);
+        }
         p.chosen = at;
         at += up256((uint64_t)bt.rows * c.heads * top * 4);
     }
@@ -184,9 +193,11 @@ gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const
     if (!std::isfinite(scale)) return invalid("token cache: scale is not finite");
     if (call.bt.rows == 0) return GVDB_OK;
     Plan p;
-    if (gvdb_status s = plan_attend(call.c, call.bt, q_heads, choose ? top : 0, p)) return s;
-    if (gvdb_status s = take_rows(q, "q", p.a.q)) return s;
-    if (gvdb_status s = take_rows(out, "out", p.a.out)) return s;
+    KvRows qr, orow;
+    if (gvdb_status s = take_rows(q, "q", qr)) return s;
+    if (gvdb_status s = take_rows(out, "out", orow)) return s;
+    if (gvdb_status s = plan_attend(call.c, call.bt, qr.dtype, q_heads, choose ? top : 0, p)) return s;
+    p.a.q = qr, p.a.out = orow;
     if (p.a.q.dtype != p.a.out.dtype) return invalid("token cache: q and out are of one dtype");
     if (p.bytes && !scratch) return invalid("token cache: null scratch");
     if (scratch_bytes < p.bytes) return invalid("token cache: scratch below gvdb_kv_scratch_bytes");
@@ -263,9 +274,11 @@ gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batc
         if (gvdb_status s = take_cache(cache, c)) return s;
         if (gvdb_status s = take_batch(batch, c, bt)) return s;
         if (bt.rows == 0) return GVDB_OK;
-        Plan p;
-        if (gvdb_status s = plan_attend(c, bt, q_heads, top, p)) return s;
-        *bytes = p.bytes;
+        for (uint32_t dtype : {GVDB_F32, GVDB_BF16}) {  // enough for either
+            Plan p;
+            if (gvdb_status s = plan_attend(c, bt, dtype, q_heads, top, p)) return s;
+            *bytes = std::max(*bytes, p.bytes);
+        }
         return GVDB_OK;
     });
 }

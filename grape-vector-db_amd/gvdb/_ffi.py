@@ -32,6 +32,7 @@ GVDB_METRIC_COSINE_DISTANCE = 2
 GVDB_SEARCH_BQ_RERANK = 0
 GVDB_SEARCH_FLAT = 1
 GVDB_F32, GVDB_F16, GVDB_BF16 = 0, 1, 2
+GVDB_KV_ZERO_REST = 1
 GVDB_N_POISONED = 0xFFFFFFFF
 GVDB_COMM_ID_BYTES = 128
 
@@ -126,7 +127,7 @@ class gvdb_kv_rows(C.Structure):
         ("row_stride", C.c_int64),
         ("head_stride", C.c_int64),
         ("dtype", C.c_uint32),
-        ("reserved", C.c_uint32),
+        ("flags", C.c_uint32),
     ]
 
 

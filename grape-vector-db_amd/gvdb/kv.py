@@ -87,7 +87,7 @@ class KvCache:
     # -- arguments ----------------------------------------------------------
     # A step's calls are shorter on the device than in Python: the C structs are packed as bytes (a third of a ctypes
     # Structure's time), and a size's scratch is asked for once.
-    def _rows(self, t, what: str, heads: int, rows: int) -> bytes:
+    def _rows(self, t, what: str, heads: int, rows: int, flags: int = 0) -> bytes:
         shape, stride = t.shape, t.stride()
         if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self.head_dim:
             raise InvalidArgument(f"{what} is [{rows}, {heads}, {self.head_dim}]: got {tuple(shape)}")
@@ -98,7 +98,7 @@ class KvCache:
             raise InvalidArgument(f"{what} is on {t.device}, the cache on {self.device}")
         if stride[2] != 1:
             raise InvalidArgument(f"{what}'s neighbouring channels lie side by side")
-        return _ROWS(t.data_ptr(), stride[0], stride[1], code, 0)
+        return _ROWS(t.data_ptr(), stride[0], stride[1], code, flags)
 
     def _batch(self, page_table, lengths, cu, rows: int, max_new: int, max_len: int):
         """(struct, sizes): the sizes are all that a call's scratch goes by."""
@@ -142,14 +142,13 @@ class KvCache:
              stream: Optional[int] = None) -> Tuple:
         """The stored keys and values of the tokens that an append of ``rows`` rows with the same arguments writes.
         Rows behind the last sequence are left as they were in ``out``, and are 0 without it."""
-        torch = self._torch
+        torch, flags = self._torch, 0
         if out is None:
-            make = torch.empty if cu is None else torch.zeros
-            shape = (rows, self.kv_heads, self.head_dim)
+            shape, flags = (rows, self.kv_heads, self.head_dim), _ffi.GVDB_KV_ZERO_REST
             dtype = dtype or torch.bfloat16
-            out = (make(shape, dtype=dtype, device=self.device), make(shape, dtype=dtype, device=self.device))
-        kr = self._rows(out[0], "out[0]", self.kv_heads, rows)
-        vr = self._rows(out[1], "out[1]", self.kv_heads, rows)
+            out = (torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device))
+        kr = self._rows(out[0], "out[0]", self.kv_heads, rows, flags)
+        vr = self._rows(out[1], "out[1]", self.kv_heads, rows, flags)
         bt, _ = self._batch(page_table, lengths, cu, rows, max_new, 0)
         status = self._lib.gvdb_kv_read_device(self._ref, bt, kr, vr, self._stream(stream))
         if status:
@@ -162,11 +161,10 @@ class KvCache:
         if len(shape) != 3:
             raise InvalidArgument("q is [rows, heads, head_dim]")
         rows, heads = shape[0], shape[1]
-        qr = self._rows(q, "q", heads, rows)
-        if out is None:
-            # rows behind the last sequence are not written: without `out` they read 0
-            out = torch.empty_like(q) if cu is None else torch.zeros_like(q)
-        orow = self._rows(out, "out", heads, rows)
+        qr, flags = self._rows(q, "q", heads, rows), 0
+        if out is None:  # rows behind the last sequence read 0; in a given `out` they stay what they were
+            out, flags = torch.empty_like(q), _ffi.GVDB_KV_ZERO_REST
+        orow = self._rows(out, "out", heads, rows, flags)
         if lse is not None and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.get_device() != self._index
                                 or not lse.is_contiguous()):
             raise InvalidArgument("lse is a contiguous float32 [rows, heads] on the cache's device")
@@ -205,12 +203,13 @@ class KvCache:
         torch = self._torch
         if top < 1 or first < 0 or recent < 0 or first + recent > top:
             raise InvalidArgument("top is at least 1 and at least first + recent, which are not negative")
+        shape = (q.shape[0], self.kv_heads, top)
+        if out is not None and chosen is None and cu is not None:  # its rows behind the last sequence are left alone as out's are
+            chosen = torch.full(shape, -1, dtype=torch.int32, device=self.device)
         heads, qr, orow, bt, scale, out, scratch, size = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out,
                                                                            lse, top)
-        shape = (q.shape[0], self.kv_heads, top)
         if chosen is None:
-            chosen = torch.empty(shape, dtype=torch.int32, device=self.device) if cu is None else torch.full(
-                shape, -1, dtype=torch.int32, device=self.device)
+            chosen = torch.empty(shape, dtype=torch.int32, device=self.device)
         elif tuple(chosen.shape) != shape or chosen.dtype != torch.int32 or chosen.get_device() != self._index or not chosen.is_contiguous():
             raise InvalidArgument("chosen is a contiguous int32 [rows, kv_heads, top] on the cache's device")
         status = self._lib.gvdb_kv_attend_topk_device(self._ref, bt, qr, heads, scale, top, first, recent, orow, chosen.data_ptr(),

@@ -573,13 +573,17 @@ typedef struct gvdb_kv_batch {
     uint32_t reserved;
 } gvdb_kv_batch;
 
+/* Output rows of no sequence become 0 (their lse -inf, their chosen pages -1)
+ * instead of staying what they were. */
+#define GVDB_KV_ZERO_REST 1u
+
 /* [rows][heads][head_dim] on the device, neighbouring channels side by side. */
 typedef struct gvdb_kv_rows {
     void* data;
     int64_t row_stride;        /* elements */
     int64_t head_stride;
     uint32_t dtype;            /* gvdb_dtype */
-    uint32_t reserved;
+    uint32_t flags;            /* outputs: 0 or GVDB_KV_ZERO_REST */
 } gvdb_kv_rows;
 
 /* Quantises rows k and v into tokens lengths[s] .. of each sequence and makes

@@ -376,6 +376,30 @@ def test_attend_topk(kv, dtype, Hq, heads, D, page, lens, new, top, first, recen
         check_attend(st, q, new, o2, chosen=got)
 
 
+@pytest.mark.parametrize("pages,new", [(700, 3), (4500, 1), (4500, 2), (16000, 1)])
+def test_topk_of_long_tables(kv, pages, new):
+    """Few pages in the pool, many in the table: scores in LDS or in memory, and many that are equal."""
+    D, page, top = 64, 32, 9
+    rng = np.random.default_rng(30)
+    st = Store(kv, 31, "bf16", 1, D, page, (page * 50,))
+    order = rng.integers(0, 50, pages)
+    table = st.table[:, torch.from_numpy(order).cuda()].contiguous()
+    length = pages * page - 5
+    long = Store.__new__(Store)
+    long.__dict__.update(st.__dict__, lens=[length])
+    rows = (order[:, None] * page + np.arange(page)).reshape(-1)[:length]
+    long.k, long.v = [st.k[0][rows]], [st.v[0][rows]]
+    q = queries(32, "bf16", (new,), 3, D).cuda()
+    out, chosen = st.cache.attend_topk(q, table, i32([length]), top, first=1, recent=2, max_len=length)
+    got = chosen.cpu().numpy()
+    fifty = st.bounds(0, 0)
+    for i in range(new):
+        seen = (length - new + i) // page + 1
+        want = plain.choose(q[i].double().cpu().numpy(), [fifty[j] for j in order], seen, top, 1, 2)
+        assert got[i, 0].tolist() == want
+    check_attend(long, q, (new,), out, chosen=got)
+
+
 def test_topk_ties_take_the_lowest_page(kv):
     """Equal pages score alike: the lowest of them are taken; all-zero queries and keys too."""
     D, page = 64, 32

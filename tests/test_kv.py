@@ -96,7 +96,7 @@ def test_batch_refusals(call, field, value):
 def test_row_refusals(call):
     from gvdb import _ffi
 
-    for field, value in (("data", None), ("dtype", 3), ("data", 4097)):
+    for field, value in (("data", None), ("dtype", 3), ("data", 4097), ("flags", 2)):
         keep = getattr(call.rows, field)
         setattr(call.rows, field, value)
         assert call.append() == ARG and call.why()
