@@ -17,6 +17,8 @@
 // S^T = K Q^T leaves lane 16 q + n with tokens 8q + 2r + i of query row n, which
 // is what O^T = V^T P^T wants of its second operand: the probabilities never
 // leave their lane, and every lane keeps the statistics of one query row.
+#include <algorithm>
+
 #include "gvdb_device.h"
 #include "gvdb_kv.h"
 
@@ -34,7 +36,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLowest = -1e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
+constexpr float kLowest = -3e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
 // Pieces of 8 bits that a type's values are split into for the products.
 constexpr int pieces(int dtype) { return dtype == GVDB_BF16 ? 1 : dtype == GVDB_F16 ? 2 : 3; }
 // The value, as one that the compiler knows nothing of: what is reckoned from it in a branch that is seldom taken stays in
@@ -843,7 +845,8 @@ __device__ __forceinline__ void clear(Rows<D, NP>& w) {
 
 template <int D>
 struct JoinLds {
-    float o[4][16][D], m[4][16], l[4][16];
+    float o[4][16][D + 4];  // rows four banks apart
+    float m[4][16], l[4][16];
 };
 
 // A row's output: sums over the row's keys, or over a part of them (`part`: its place among the parts).
@@ -871,26 +874,33 @@ template <int D, int T, int NP, bool CHOSEN>
 __device__ __forceinline__ void join_waves(JoinLds<D>& s, Rows<D, NP>& w, const Job<CHOSEN>& j, const AttendArgs& a, uint32_t split) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, q4 = lane >> 4, n16 = lane & 15u;
     w.l = row_sum(w.l);
-    if (q4 == 0) s.m[wave][n16] = w.m, s.l[wave][n16] = w.l;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(s.m[0][n16], s.m[1][n16]), fmaxf(s.m[2][n16], s.m[3][n16]));
-    const float f = __builtin_amdgcn_exp2f(w.m - top);
+    if (j.token >= 0) {  // the lane's channels: r * (D / 16) + k behind q4 * (D / 4)
+        if (q4 == 0) s.m[wave][n16] = w.m, s.l[wave][n16] = w.l;
+        f4* to = (f4*)&s.o[wave][n16][q4 * (D / 4)];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int c = 0; c < D / 16; ++c) {
+            f4 x;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) s.o[wave][n16][q4 * (D / 4) + r * (D / 16) + k] = w.o[k][r] * f;
+            for (int i = 0; i < 4; ++i) x[i] = w.o[(4 * c + i) % (D / 16)][(4 * c + i) / (D / 16)];
+            to[c] = x;
+        }
+    }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < 16 * (D / 8); e += 256) {
+    const uint32_t live = (uint32_t)min(16, j.rows - j.first);
+#pragma unroll 1
+    for (uint32_t e = threadIdx.x; e < live * (D / 8); e += 256) {
         const uint32_t r = e / (D / 8), d = e % (D / 8) * 8;
-        const int row = j.first + (int)r;
-        if (row >= j.rows) continue;
         const float m = fmaxf(fmaxf(s.m[0][r], s.m[1][r]), fmaxf(s.m[2][r], s.m[3][r]));
-        float l = 0.f;
+        float l = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) l += s.l[k][r] * __builtin_amdgcn_exp2f(s.m[k][r] - m);
-        float x[8];
+        for (int k = 0; k < 4; ++k) {
+            const float f = __builtin_amdgcn_exp2f(s.m[k][r] - m);
+            const f4 u = *(const f4*)&s.o[k][r][d], v = *(const f4*)&s.o[k][r][d + 4];
+            l += s.l[k][r] * f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (s.o[0][r][d + i] + s.o[1][r][d + i]) + (s.o[2][r][d + i] + s.o[3][r][d + i]);
+            for (int i = 0; i < 4; ++i) x[i] += u[i] * f, x[4 + i] += v[i] * f;
+        }
+        const int row = j.first + (int)r;
         write_row<D, T>(a, j, row, d, x, m, l, a.splits > 1,
                         ((uint64_t)j.token_of(row) * a.q_heads + j.head_of(row)) * a.splits + split);
     }
@@ -1527,11 +1537,11 @@ __device__ __forceinline__ void score_pages(const u4 (&pb)[D / 32], uint32_t e, 
     for (int r = 0; r < 4; ++r) best[r] = be[r] == 255u ? 3.402823466e38f : best[r];
 }
 
-// Scores of pages [from, to) for 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256: half
-// of them); `put` takes four neighbouring pages' scores.
-template <int D, class Put>
-__device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt, uint32_t b, uint32_t h, const ScoreCols<D>& col, uint32_t width,
-                                            int64_t from, int64_t to, uint32_t wave, uint32_t waves, uint32_t lane, Put put) {
+// Scores of pages [from, to) for CG times 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256:
+// half of them); `put` takes four neighbouring pages' scores for the g-th 16 columns.
+template <int D, int CG, class Put>
+__device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt, uint32_t b, uint32_t h, const ScoreCols<D> (&col)[CG],
+                                            uint32_t width, int64_t from, int64_t to, uint32_t wave, uint32_t waves, uint32_t lane, Put put) {
     constexpr int NB = D == 256 ? 2 : 4;
     const uint32_t q4 = lane >> 4, n16 = lane & 15u;
     auto look = [&](int64_t p) { return p + lane < to ? (int)page_of(c, bt, b, (uint32_t)(p + lane)) : -1; };
@@ -1553,11 +1563,13 @@ __device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt,
             }
             if (s + NB == 4) page = look(p + waves * 64);
 #pragma unroll
-            for (int x = 0; x < NB; ++x) {
-                float best[4];
-                score_pages<D>(pb[x], e, 16 * (s + x), col, width, q4, best);
-                put(p + 16 * (s + x) + 4 * q4, best);
-            }
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int g = 0; g < CG; ++g) {
+                    float best[4];
+                    score_pages<D>(pb[x], e, 16 * (s + x), col[g], width, q4, best);
+                    put(g, p + 16 * (s + x) + 4 * q4, best);
+                }
         }
     }
 }
@@ -1687,9 +1699,10 @@ __device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uin
     meet();
 }
 
-// One workgroup: the pages of 16 / width tokens of a sequence (`per` of them here) and one key head, scored into LDS and chosen
-// there.  Bound by the bounds that it reads, 2 D + 1 bytes a page.
-template <int D, int T>
+// One workgroup: the pages of `per` tokens of a sequence (at most CG times 16 / width) and one key head, scored into LDS and chosen
+// there.  The tokens share the bounds that it reads, 2 D + 1 bytes a page; 384 tokens over 1024 pages take 67 us one sixteen
+// columns a workgroup.
+template <int D, int T, int CG>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t per) {
     extern __shared__ float s_sc[];  // [per][table_width]
     __shared__ ChooseLds s_choose;
@@ -1704,20 +1717,23 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
         const int toks = min((int)per, n - t0);
         const int64_t have = a.pages_seen(c, bt, before + t0 + toks - 1), seen = min(have, (int64_t)bt.table_width);
         if (have > (int64_t)a.top) {
-            const uint32_t my = n16 / width;  // this lane's token of the tile
+            const uint32_t my = n16 / width, toks16 = 16 / width;  // this lane's token of each sixteen columns
             for (uint32_t g0 = 0; g0 < group; g0 += width) {
                 const uint32_t gh = g0 + n16 % width;
-                ScoreCols<D> col;
-                col.template load<T>(a, (int)my < toks && gh < group,
-                                     (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
-                score_range<D>(c, bt, b, h, col, width, 0, seen, wave, kChooseThreads / 64, lane, [&](int64_t p, const float(&best)[4]) {
-                    if ((int)my >= toks || n16 % width) return;
+                ScoreCols<D> col[CG];
+#pragma unroll
+                for (int g = 0; g < CG; ++g) {
+                    const int tok = g * (int)toks16 + (int)my;
+                    col[g].template load<T>(a, tok < toks && gh < group,
+                                            (int64_t)(r0 + t0 + tok) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+                }
+                score_range<D, CG>(c, bt, b, h, col, width, 0, seen, wave, kChooseWaves, lane, [&](int g, int64_t p, const float(&best)[4]) {
+                    const int tok = g * (int)toks16 + (int)my;
+                    if (tok >= toks || n16 % width) return;
+                    float* to = &s_sc[tok * bt.table_width + p];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (p + r < seen) {
-                            float* to = &s_sc[my * bt.table_width + p + r];
-                            *to = g0 ? fmaxf(*to, best[r]) : best[r];
-                        }
+                        if (p + r < seen) to[r] = g0 ? fmaxf(to[r], best[r]) : best[r];
                 });
             }
         }
@@ -1762,10 +1778,10 @@ __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendA
         const uint32_t my = n16 / width;
         for (uint32_t g0 = 0; g0 < group && from < to; g0 += width) {
             const uint32_t gh = g0 + n16 % width;
-            ScoreCols<D> col;
-            col.template load<T>(a, (int)my < toks && gh < group,
-                                 (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
-            score_range<D>(c, bt, b, h, col, width, from, to, wave, 4, lane, [&](int64_t p, const float(&best)[4]) {
+            ScoreCols<D> col[1];
+            col[0].template load<T>(a, (int)my < toks && gh < group,
+                                    (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+            score_range<D, 1>(c, bt, b, h, col, width, from, to, wave, 4, lane, [&](int, int64_t p, const float(&best)[4]) {
                 if ((int)my >= toks || n16 % width) return;
                 float* out = a.scores + ((uint64_t)(r0 + t0 + (int)my) * c.heads + h) * bt.table_width + p;
 #pragma unroll
@@ -1832,7 +1848,8 @@ uint32_t capped(uint64_t n, uint64_t others, uint64_t cap) {
     const uint64_t most = cap / others + 1;
     return (uint32_t)(n < 1 ? 1 : n > most ? most : n);
 }
-bool fits(uint64_t blocks) { return blocks > 0 && blocks <= 0x7FFFFFFFull; }
+// A launch's threads along x are counted in 32 bits.
+bool fits(uint64_t blocks, uint64_t threads = 256) { return blocks > 0 && blocks * threads < (1ull << 32); }
 }  // namespace
 
 hipError_t launch_kv_append(const KvCache& c, const KvBatch& bt, const KvRows& k, const KvRows& v, hipStream_t s) {
@@ -1880,9 +1897,13 @@ hipError_t launch_kv_attend(const KvCache& c, const KvBatch& bt, const AttendArg
 
 hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const AttendArgs& a, hipStream_t s) {
     const uint32_t group = a.q_heads / c.heads;
-    uint32_t per = 16 / (group >= 16 ? 16 : next_pow2(group));
-    if (bt.max_new < per) per = next_pow2(bt.max_new);
+    const uint32_t per16 = 16 / (group >= 16 ? 16 : next_pow2(group));
     const bool fused = a.score_chunk == 0;
+    // prompts: several times 16 columns a workgroup, eight tokens, one a wave, at most
+    const uint32_t groups = c.dim == 256 ? 2 : 4;
+    const bool many = fused && bt.max_new >= 2 * per16;
+    uint32_t per = many ? std::min(groups * per16, kChooseWaves) : per16;
+    if (bt.max_new < per) per = next_pow2(bt.max_new);
     while (fused && per > 1 && per * bt.table_width > kChooseScores) per /= 2;
     const uint32_t chunks = fused ? 1 : (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
     const uint64_t others = (uint64_t)c.heads * chunks * bt.n_seqs;
@@ -1890,11 +1911,17 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
     const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.rows);
     const bool few = !a.lanes && a.splits <= 16;
     const uint64_t per_join = few ? 4 * (512 / c.dim) : 4, joins = ((uint64_t)bt.rows * a.q_heads + per_join - 1) / per_join;
-    if (!fits(others * tok_tiles) || !fits(blocks) || !fits(joins) || !fits((uint64_t)bt.rows * c.heads)) return hipErrorInvalidValue;
+    if (!fits(others * tok_tiles, kChooseThreads) || !fits(blocks) || !fits(joins) || (!fused && !fits((uint64_t)bt.rows * c.heads, kChooseThreads)))
+        return hipErrorInvalidValue;
     if (fused) {
         const uint32_t lds = per * bt.table_width * 4;
-        KV_DISPATCH(c.dim, a.q.dtype,
-                    (k_kv_choose<D, T><<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
+        if (many) {
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_choose<D, T, D == 256 ? 2 : 4>
+                                           <<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
+        } else {
+            KV_DISPATCH(c.dim, a.q.dtype,
+                        (k_kv_choose<D, T, 1><<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
+        }
         GVDB_LAUNCH_CHECK();
     } else {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));

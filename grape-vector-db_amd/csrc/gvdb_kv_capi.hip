@@ -45,6 +45,7 @@ gvdb_status launch(int device, const char* what, hipError_t (*run)(const void*, 
     hipError_t e = scope.err;
     if (e == hipSuccess) e = run(args, (hipStream_t)stream);
     if (e == hipSuccess) return GVDB_OK;
+    if (e == hipErrorInvalidValue) return invalid("token cache: more rows and heads than one launch takes");
     return report_status(e == hipErrorOutOfMemory ? GVDB_ERR_OUT_OF_MEMORY : GVDB_ERR_DEVICE,
                          std::string(what) + ": " + hipGetErrorString(e));
 }
@@ -129,10 +130,13 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     // Two workgroups a CU: four waves a SIMD pair read 5.3 TB/s.  64 sequences of up to 10000 tokens: 65 us with one, 58 with
     // two, 69 with three, 65 with four; 4 x 256K tokens: 263, 215, 231, 226 us.
     const uint64_t slots = 512;
+    // The line helps while sequences are of several lengths (250 of them, 8 heads: 94 us, whole units 102); chosen pages are of one
+    // length, and whole units win from 1024 on (384 tokens, 4 heads: 100 us, the line 103).
+    const uint64_t line_most = (top ? 2 : 8) * slots;
     a.row_tiles = (uint32_t)row_tiles;
     a.splits = 1;
     a.chunk = (uint32_t)(tiles + 1) / 2 * 2;
-    if (a.many ? busy < 2 * slots && tiles > 32 : tiles > 32 && units < 4 * slots) {  // else a workgroup takes its rows' tiles whole
+    if (a.many ? busy < 2 * slots && tiles > 32 : tiles > 32 && units < line_most) {  // else a workgroup takes its rows' tiles whole
         const uint64_t line = units0 * ((rows_each + 15) / 16);
         const uint64_t most = line * (top ? (uint64_t)top : (uint64_t)bt.table_width + 1) * (c.page / 32);
         if (!a.many && (top || !bt.cu) && line <= kMaxUnits && most < (1ull << 31)) {
@@ -151,8 +155,12 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     const uint64_t qr = (uint64_t)bt.rows * q_heads;
     uint64_t at = 0;
     if (top) {
+        // Scores go by way of memory where LDS does not hold them, and where few tokens have many pages: all CUs score, 30 us for one
+        // sequence of 1024 pages against 33 by one workgroup a head, 53 against 55 for 32 sequences; 384 tokens of a prompt take 45 us
+        // in LDS and 82 by way of memory.
         const bool split = bt.table_width > kChooseScores || (kv_max_pages(c, bt) > 512 && (uint64_t)bt.rows * c.heads <= 1024);
-        a.score_chunk = split ? 256 : 0;
+        // 256 pages a workgroup, 64 a wave; 128 where that leaves CUs idle (one sequence of 1024 pages, 8 heads: 31 and 29 us)
+        a.score_chunk = !split ? 0 : (uint64_t)bt.rows * c.heads * kv_max_pages(c, bt) < 65536 ? 128 : 256;
         if (split) {
             p.scores = at;
             at += up256((uint64_t)bt.rows * c.heads * bt.table_width * 4);

@@ -36,7 +36,8 @@ class KvCache:
     [sequences, width]: each sequence's pages in token order.  A row tensor is
     [rows, heads, head_dim] in bf16, f16 or f32 with neighbouring channels side by
     side; its rows belong to the sequences by ``cu`` (int32 [sequences + 1]), or
-    evenly without it.  ``max_new`` (most rows of one sequence) and ``max_len`` (the
+    evenly without it.  ``stream`` (a HIP stream's handle) runs a call there instead of
+    on torch's current stream.  ``max_new`` (most rows of one sequence) and ``max_len`` (the
     largest length) size the launch and change no result.
     """
 
@@ -122,19 +123,25 @@ class KvCache:
         return (_BATCH(page_table.data_ptr(), stride[0], width, n, lengths.data_ptr(), at, rows, max_new, max_len, 0),
                 (rows, n, width, at != 0, max_new, max_len))
 
-    def _stream(self, stream: Optional[int]):
-        if stream is not None:
-            return stream or None
+    def _stream(self):
         return self._raw_stream(self._index) or None
+
+    def _on(self, stream: int):
+        """Torch's current stream made the given one: what a call allocates belongs to the stream that it runs on."""
+        cuda = self._torch.cuda
+        return cuda.stream(cuda.ExternalStream(stream, device=self.device) if stream else cuda.default_stream(self.device))
 
     # -- operators ----------------------------------------------------------
     def append(self, k, v, page_table, lengths, cu=None, max_new: int = 0, stream: Optional[int] = None) -> None:
         """Writes rows ``k`` and ``v`` as tokens ``lengths[s]`` .. of each sequence (``lengths``: tokens before the call)."""
+        if stream is not None:
+            with self._on(stream):
+                return self.append(k, v, page_table, lengths, cu, max_new)
         rows = k.shape[0]
         kr = self._rows(k, "k", self.kv_heads, rows)
         vr = self._rows(v, "v", self.kv_heads, rows)
         bt, _ = self._batch(page_table, lengths, cu, rows, max_new, 0)
-        status = self._lib.gvdb_kv_append_device(self._ref, bt, kr, vr, self._stream(stream))
+        status = self._lib.gvdb_kv_append_device(self._ref, bt, kr, vr, self._stream())
         if status:
             check(status)
 
@@ -142,6 +149,9 @@ class KvCache:
              stream: Optional[int] = None) -> Tuple:
         """The stored keys and values of the tokens that an append of ``rows`` rows with the same arguments writes.
         Rows behind the last sequence are left as they were in ``out``, and are 0 without it."""
+        if stream is not None:
+            with self._on(stream):
+                return self.read(page_table, lengths, rows, cu, max_new, dtype, out)
         torch, flags = self._torch, 0
         if out is None:
             shape, flags = (rows, self.kv_heads, self.head_dim), _ffi.GVDB_KV_ZERO_REST
@@ -150,7 +160,7 @@ class KvCache:
         kr = self._rows(out[0], "out[0]", self.kv_heads, rows, flags)
         vr = self._rows(out[1], "out[1]", self.kv_heads, rows, flags)
         bt, _ = self._batch(page_table, lengths, cu, rows, max_new, 0)
-        status = self._lib.gvdb_kv_read_device(self._ref, bt, kr, vr, self._stream(stream))
+        status = self._lib.gvdb_kv_read_device(self._ref, bt, kr, vr, self._stream())
         if status:
             check(status)
         return out
@@ -186,10 +196,13 @@ class KvCache:
         """Attention of rows ``q`` over their sequences' tokens (``lengths``: with the call's own).  With ``causal``, row i of a
         sequence's n sees the first ``length - n + i + 1`` tokens.  ``scale``: 1 / sqrt(head_dim) by default; ``lse``
         [rows, heads] float32 takes the logarithm of the softmax's denominator.  A row that sees nothing is 0."""
+        if stream is not None:
+            with self._on(stream):
+                return self.attend(q, page_table, lengths, cu, max_new, max_len, scale, causal, out, lse)
         heads, qr, orow, bt, scale, out, scratch, size = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out,
                                                                            lse, 0)
         status = self._lib.gvdb_kv_attend_device(self._ref, bt, qr, heads, scale, 1 if causal else 0, orow, _ffi.ptr(lse),
-                                                 _ffi.ptr(scratch), size, self._stream(stream))
+                                                 _ffi.ptr(scratch), size, self._stream())
         if status:
             check(status)
         return out
@@ -200,6 +213,9 @@ class KvCache:
         """Causal attention over ``top`` pages of each row and key/value head: the ``first`` first, the ``recent`` last, and
         those whose key bounds promise the largest scores.  Returns ``(out, chosen)``; ``chosen`` is int32 [rows, kv_heads,
         top], positions in the page table in order, -1 behind the last."""
+        if stream is not None:
+            with self._on(stream):
+                return self.attend_topk(q, page_table, lengths, top, first, recent, cu, max_new, max_len, scale, out, chosen, lse)
         torch = self._torch
         if top < 1 or first < 0 or recent < 0 or first + recent > top:
             raise InvalidArgument("top is at least 1 and at least first + recent, which are not negative")
@@ -213,7 +229,7 @@ class KvCache:
         elif tuple(chosen.shape) != shape or chosen.dtype != torch.int32 or chosen.get_device() != self._index or not chosen.is_contiguous():
             raise InvalidArgument("chosen is a contiguous int32 [rows, kv_heads, top] on the cache's device")
         status = self._lib.gvdb_kv_attend_topk_device(self._ref, bt, qr, heads, scale, top, first, recent, orow, chosen.data_ptr(),
-                                                      _ffi.ptr(lse), _ffi.ptr(scratch), size, self._stream(stream))
+                                                      _ffi.ptr(lse), _ffi.ptr(scratch), size, self._stream())
         if status:
             check(status)
         return out, chosen

@@ -220,6 +220,9 @@ def test_pages_that_are_not_there(kv):
     assert np.array_equal(k.double().cpu().numpy()[~bad], want[~bad])
     q = torch.randn(6, 2, D, device="cuda")
     for lens, nan in (((33, 64, 96), (0,)), ((32, 65, 96), (1,)), ((32, 64, 97), (2,))):
+        many = q.to(torch.bfloat16).view(3, 2, 2, D).repeat_interleave(40, 1).view(240, 2, D).contiguous()  # 160 rows a sequence
+        wide = c.attend(many, table, i32(lens)).view(3, 80, 2, D)
+        assert torch.isnan(wide[:, -1]).flatten(1).all(1).tolist() == [s in nan for s in range(3)]
         for o in (c.attend(q, table, i32(lens)), c.attend_topk(q, table, i32(lens), 3)[0]):
             got = torch.isnan(o).flatten(1).all(1).cpu().view(3, 2)[:, 1].nonzero().flatten().tolist()
             assert got == list(nan), (lens, got)
@@ -250,7 +253,7 @@ def test_attend(kv, dtype, Hq, heads, D, page, lens, new):
     check_attend(st, q, new, out, lse)
     if len(set(new)) == 1:  # without cu the keys may be cut elsewhere: another order of the same sums, under the same bound
         check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), max_len=max(lens)))
-    # hints size the launch only: too small, too large and none give the same sums up to their order
+    # hints size the launch only: too small, too large and none give the same sums, in another order
     for hints in ({"max_new": 1, "max_len": 1}, {}, {"max_new": 10 ** 6, "max_len": 10 ** 6}):
         check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), cu=cu, **hints))
 
@@ -285,39 +288,113 @@ def test_attend_sharp_and_flat(kv, dtype, spread):
     check_attend(st, q, (3,), st.cache.attend(q, st.table, st.lengths()))
 
 
-def test_what_is_masked_may_hold_anything(kv):
+@pytest.mark.parametrize("dtype,heads,Hq,D,page", [("f32", 1, 2, 128, 64), ("bf16", 1, 2, 128, 64), ("f16", 1, 2, 64, 32), ("bf16", 2, 4, 256, 96)])
+def test_what_is_masked_may_hold_anything(kv, dtype, heads, Hq, D, page):
     """A key or value that is not finite shows in the rows that see it, and in no other; a value only in its group of channels."""
-    D, page = 128, 64
     for poison in (float("nan"), float("inf"), -float("inf")):
-        st = Store(kv, 10, "f32", 1, D, page, (150,))
-        k = torch.from_numpy(np.random.default_rng(1).standard_normal((4, 1, D))).float().cuda()
+        st = Store(kv, 10, dtype, heads, D, page, (150,))
+        k = torch.from_numpy(np.random.default_rng(1).standard_normal((4, heads, D))).to(DT[dtype]).cuda()
         v = k.clone()
-        v[1, 0, 40] = poison   # token 121: a value, channels 32 .. 63
-        k[3, 0, 7] = poison    # token 123: a key
+        v[1, :, 40] = poison   # token 121: a value, channels 32 .. 63
+        k[3, :, 7] = poison    # token 123: a key
         st.cache.append(k, v, st.table, i32([120]))
         st.k[0][120:124], st.v[0][120:124] = plain.stored(k.double().cpu().numpy()), plain.stored(v.double().cpu().numpy())
-        q = queries(11, "f32", (150,), 2, D).cuda()
-        lse = torch.empty(150, 2, device="cuda")
+        q = queries(11, dtype, (150,), Hq, D).cuda()
+        lse = torch.empty(150, Hq, device="cuda")
         out = st.cache.attend(q, st.table, st.lengths(), lse=lse)
         nan = torch.isnan(out).cpu().numpy()
-        want = np.zeros((150, 2, D), bool)
+        want = np.zeros((150, Hq, D), bool)
         want[121:, :, 32:64] = True
         want[123:] = True
         assert np.array_equal(nan, want)
-        skip = {(r, h) for r in range(121, 150) for h in range(2)}
+        skip = {(r, h) for r in range(121, 150) for h in range(Hq)}
         check_attend(st, q, (150,), out, skip=skip)
+        # the channels beside the value's group are what they would be
+        got = out.double().cpu().numpy()[121:123]
+        for r in range(2):
+            for hq in range(Hq):
+                h = hq // (Hq // heads)
+                n = 122 + r
+                vv = np.nan_to_num(st.v[0][:n, h])
+                o, _, absum, _ = plain.attend(q[121 + r, hq].double().cpu().numpy(), st.k[0][:n, h], vv, D ** -0.5, np.ones(n, bool))
+                other = np.r_[0:32, 64:D]
+                assert (np.abs(got[r, hq] - o)[other] <= (HALF[dtype] * np.abs(o) + 2 * (PROB[dtype] + 2.0 ** -12) * absum)[other]).all()
         # single tokens over a shorter length
         for n, bad in ((121, False), (122, True), (124, True)):
             one = st.cache.attend(q[:1], st.table, i32([n]))
             assert bool(torch.isnan(one).any()) == bad
             assert bool(torch.isnan(one).all()) == (n == 124)
-    # a query that is not finite spoils its own row alone
-    st = Store(kv, 12, "bf16", 2, 64, 32, (80, 80))
-    q = queries(13, "bf16", (2, 2), 4, 64).cuda()
-    q[1, 2, 5] = float("nan")
-    out = st.cache.attend(q, st.table, st.lengths())
-    assert torch.isnan(out[1, 2]).all()
-    check_attend(st, q, (2, 2), out, skip={(1, 2)})
+
+
+def test_a_query_that_is_not_finite_spoils_its_own_row(kv):
+    for new, Hq in (((2, 2), 4), ((70, 66), 4)):
+        st = Store(kv, 12, "bf16", 2, 64, 32, (80, 80))
+        q = queries(13, "bf16", new, Hq, 64).cuda()
+        q[1, 2, 5] = float("nan")
+        q[new[0], 0, 0] = float("inf")
+        out = st.cache.attend(q, st.table, st.lengths(), cu=i32([0, new[0], sum(new)]))
+        assert torch.isnan(out[1, 2]).all() and torch.isnan(out[new[0], 0]).all()
+        check_attend(st, q, new, out, skip={(1, 2), (new[0], 0)})
+
+
+@pytest.mark.parametrize("dtype,Hq,heads,D,page,lens,new,causal", [
+    ("bf16", 8, 2, 64, 32, (400, 70, 9), (33, 70, 40), True),     # the last sequence is shorter than its rows
+    ("f16", 8, 2, 128, 64, (500, 0), (200, 3), False),
+    ("bf16", 4, 2, 256, 64, (300,), (129,), True),
+    ("f16", 3, 1, 256, 1024, (1300,), (47,), True),
+    ("bf16", 64, 1, 64, 64, (4000,), (5,), True),                 # few rows blocks: split along the keys
+    ("f16", 32, 2, 128, 96, (3000, 2500), (8, 9), True),
+])
+def test_attend_many_rows(kv, dtype, Hq, heads, D, page, lens, new, causal):
+    st = Store(kv, 40, dtype, heads, D, page, lens)
+    q = queries(41, dtype, new, Hq, D).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), cu=i32(np.cumsum((0,) + new).tolist()), causal=causal, lse=lse, max_new=max(new))
+    check_attend(st, q, new, out, lse, causal=causal)
+
+
+def test_rows_outside_every_sequence(kv):
+    """cu may begin behind the first row and end before the last: those rows are left alone, or 0 where the call makes the output."""
+    D, Hq, heads = 64, 4, 2
+    for new, dtype in (((3, 2), "f32"), ((70, 40), "bf16")):
+        st = Store(kv, 42, dtype, heads, D, 32, (100, 90))
+        q = queries(43, dtype, (2 + sum(new) + 3,), Hq, D).cuda()
+        cu = i32([2, 2 + new[0], 2 + sum(new)])
+        rest = [0, 1] + list(range(2 + sum(new), 5 + sum(new)))
+        for given in (False, True):
+            keep = torch.full_like(q, 9.0) if given else None
+            out = st.cache.attend(q, st.table, st.lengths(), cu=cu, out=keep)
+            got, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 2, cu=cu, out=keep.clone() if given else None)
+            for o in (out, got):
+                assert (o[rest] == (9 if given else 0)).all()
+            assert (chosen[rest] == -1).all()
+            check_attend(st, q[2:-3], new, out[2:-3])
+            check_attend(st, q[2:-3], new, got[2:-3], chosen=chosen[2:-3].cpu().numpy())
+        k, v = st.cache.read(st.table, st.zeros(), q.shape[0], cu=cu, dtype=torch.float32)
+        assert (k[rest] == 0).all() and (v[rest] == 0).all() and torch.isfinite(k).all()
+        assert np.array_equal(k[2:2 + new[0]].double().cpu().numpy(), st.k[0][:new[0]])
+
+
+def test_pools_over_32_bits(kv):
+    """Pages whose bytes lie behind 4 GiB."""
+    D, heads, page, n = 256, 8, 64, 40000
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GiB")
+    c = kv.KvCache(n, heads, D, page)
+    assert c.pool.numel() > 5 << 30
+    table = i32([[n - 1, 3, n - 7, 35000, 0]])
+    x, y = (torch.randn(300, heads, D, device="cuda") for _ in range(2))
+    c.append(x, y, table, i32([0]))
+    k, v = c.read(table, i32([0]), 300, dtype=torch.float32)
+    assert np.array_equal(k.double().cpu().numpy(), plain.stored(x.double().cpu().numpy()))
+    assert np.array_equal(v.double().cpu().numpy(), plain.stored(y.double().cpu().numpy()))
+    st = Store.__new__(Store)
+    st.__dict__.update(cache=c, table=table, lens=[300], page=page, heads=heads, D=D, dtype="f32", k=[k.double().cpu().numpy()],
+                       v=[v.double().cpu().numpy()])
+    q = queries(44, "f32", (2,), heads, D).cuda()
+    check_attend(st, q, (2,), c.attend(q, table, i32([300])))
+    out, chosen = c.attend_topk(q, table, i32([300]), 3)
+    check_attend(st, q, (2,), out, chosen=chosen.cpu().numpy())
 
 
 def test_strided_misaligned_and_given_outputs(kv):
@@ -348,6 +425,9 @@ def test_strided_misaligned_and_given_outputs(kv):
     ("bf16", 3, 1, 128, 128, (2000, 7, 30), (9, 7, 40), 3, 1, 1),
     ("f16", 4, 4, 128, 32, (500,), (40,), 100, 1, 1),     # more than there are: everything
     ("bf16", 4, 2, 64, 32, (300, 200), (1, 1), 1, 0, 1),
+    ("f16", 4, 1, 256, 32, (600,), (20,), 5, 1, 1),       # prompts: several times 16 columns share the bounds
+    ("f32", 14, 2, 64, 32, (900, 33), (21, 12), 6, 2, 1),
+    ("bf16", 34, 2, 128, 32, (800,), (7,), 70, 1, 3),     # more heads a group than columns, more pages than a wave has lanes
 ])
 def test_attend_topk(kv, dtype, Hq, heads, D, page, lens, new, top, first, recent):
     st = Store(kv, 15, dtype, heads, D, page, lens)
@@ -472,6 +552,17 @@ def test_another_stream(kv):
         gk, gc = st.cache.attend_topk(q, st.table, lens, 6)
     side.synchronize()
     assert torch.equal(got, want) and torch.equal(gk, wk) and torch.equal(gc, wc)
+    # by handle, while the current stream allocates and writes: no call's scratch is handed to another stream
+    other = torch.cuda.Stream()
+    outs = []
+    for _ in range(20):
+        outs.append(st.cache.attend(q, st.table, lens, stream=other.cuda_stream))
+        outs.append(st.cache.attend_topk(q, st.table, lens, 6, stream=other.cuda_stream)[0])
+        junk = [torch.full((1 << 16,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        del junk
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want if i % 2 == 0 else wk) for i, o in enumerate(outs))
+    assert torch.equal(st.cache.attend(q, st.table, lens, stream=0), want)
 
 
 def test_captured_and_replayed(kv):
