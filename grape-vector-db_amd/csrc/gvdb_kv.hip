@@ -656,8 +656,8 @@ __device__ __forceinline__ void settle_tile(Rows<D, NP>& w, Tile<D>& t, f4 (&s)[
 }
 
 // Adds a tile's values by the probabilities pf.
-template <int D, int NP>
-__device__ __forceinline__ void tile_values(Rows<D, NP>& w, const Tile<D>& t, const u4 (&pf)[NP]) {
+template <int D, int NP, int PP>
+__device__ __forceinline__ void tile_values(Rows<D, NP>& w, const Tile<D>& t, const u4 (&pf)[PP]) {
     float vs[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) vs[e] = bits_f32((t.vs[e / 4] >> (8 * (e % 4)) & 255u) << 23);
@@ -672,7 +672,7 @@ __device__ __forceinline__ void tile_values(Rows<D, NP>& w, const Tile<D>& t, co
             odd[r] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
+        for (int p = 0; p < PP; ++p) {
             w.o[2 * jb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(even), as_bf8(pf[p]), w.o[2 * jb], 0, 0, 0);
             w.o[2 * jb + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(odd), as_bf8(pf[p]), w.o[2 * jb + 1], 0, 0, 0);
         }
@@ -689,6 +689,7 @@ struct Step {  // tiles whose loads were issued together
 // One step for 16 rows: the running maximum and sum of a softmax over its NT * 32 tokens.
 template <int D, int NP, bool CHOSEN, int NT>
 __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const Job<CHOSEN>& j, float c2, uint32_t lane) {
+    constexpr int PP = NP < 2 ? 2 : NP;  // of a probability: with one, half of a bf16 row's error would be the probabilities'
     f4 s[NT][2];
     uint32_t odd = 0;
     bool plain = true;
@@ -723,18 +724,18 @@ __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const
     }
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-        u4 pf[NP];
+        u4 pf[PP];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][0][e], c2, -top));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][1][e], c2, -top));
-            uint32_t pc[NP];
-            pack_pieces<NP>(p0, p1, pc);
+            uint32_t pc[PP];
+            pack_pieces<PP>(p0, p1, pc);
             w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
 #pragma unroll
-            for (int p = 0; p < NP; ++p) pf[p][e] = pc[p];
+            for (int p = 0; p < PP; ++p) pf[p][e] = pc[p];
         }
-        tile_values<D, NP>(w, st.t[x], pf);
+        tile_values<D, NP, PP>(w, st.t[x], pf);
     }
 }
 
@@ -1103,8 +1104,10 @@ __device__ __forceinline__ void load_keys32(const uint8_t* p, uint32_t i, uint32
 }
 
 // Rows of 16 bits only: in 32 bits the pieces of 32 rows do not fit the registers.
+// Probabilities of bf16 rows are in one piece here, where a second one's products would cost a third of the time; the bound on
+// workgroups keeps D = 64 within a third of the registers (55 -> 52 us: 2 sequences of up to 500 tokens, f16).
 template <int D, int T>
-__global__ __launch_bounds__(256, D < 256 ? 2 : 1) void k_kv_attend_rows(KvCache c, KvBatch bt, AttendArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_attend_rows(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T), W = D / 16, G = D / 32;
     __shared__ u4 s_v[2][8 * D];
     __shared__ uint32_t s_odd[2][4];

@@ -147,7 +147,10 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
             a.slot_rows = (uint32_t)std::min<uint64_t>(16, rows_each);
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
         } else {
-            a.chunk = (uint32_t)std::max<uint64_t>(a.many ? 16 : 8, ((busy * tiles + 2 * slots - 1) / (2 * slots) + 1) / 2 * 2);  // whole steps
+            // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 336 us,
+            // for 1024 of them 354, for 512 432), or 768 of 16 rows (up to 5 tokens of 8 sequences over 20000: 37 us, for 512 47)
+            const uint64_t parts = a.many ? 4 * slots : slots + slots / 2;
+            a.chunk = (uint32_t)std::max<uint64_t>(a.many ? 16 : 8, ((busy * tiles + parts - 1) / parts + 1) / 2 * 2);  // whole steps
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         }
     }
