@@ -99,6 +99,15 @@ gvdb_status take_rows(const gvdb_kv_rows* in, const char* what, KvRows& r) {
     return GVDB_OK;
 }
 
+// Rows that are written lie apart: two that share an element would be written in any order.
+gvdb_status take_out(const gvdb_kv_rows* in, const char* what, const KvCache& c, uint32_t rows, uint32_t heads, KvRows& r) {
+    if (gvdb_status s = take_rows(in, what, r)) return s;
+    const int64_t d = c.dim;
+    if ((rows > 1 && r.row_stride > -d && r.row_stride < d) || (heads > 1 && r.head_stride > -d && r.head_stride < d))
+        return invalid((std::string("token cache: overlapping rows of ") + what).c_str());
+    return GVDB_OK;
+}
+
 uint64_t up256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 // How the work is cut, and where in the scratch each part lies.
@@ -206,7 +215,7 @@ gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const
     Plan p;
     KvRows qr, orow;
     if (gvdb_status s = take_rows(q, "q", qr)) return s;
-    if (gvdb_status s = take_rows(out, "out", orow)) return s;
+    if (gvdb_status s = take_out(out, "out", call.c, call.bt.rows, q_heads, orow)) return s;
     if (gvdb_status s = plan_attend(call.c, call.bt, qr.dtype, q_heads, choose ? top : 0, p)) return s;
     p.a.q = qr, p.a.out = orow;
     if (p.a.q.dtype != p.a.out.dtype) return invalid("token cache: q and out are of one dtype");
@@ -265,9 +274,9 @@ gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch*
         if (gvdb_status s = take_batch(batch, call.c, call.bt)) return s;
         if (call.bt.rows == 0 || (!k && !v)) return GVDB_OK;
         if (k)
-            if (gvdb_status s = take_rows(k, "k", call.k)) return s;
+            if (gvdb_status s = take_out(k, "k", call.c, call.bt.rows, call.c.heads, call.k)) return s;
         if (v)
-            if (gvdb_status s = take_rows(v, "v", call.v)) return s;
+            if (gvdb_status s = take_out(v, "v", call.c, call.bt.rows, call.c.heads, call.v)) return s;
         if (k && v && call.k.dtype != call.v.dtype) return invalid("token cache: k and v are of one dtype");
         return launch(cache->device, "kv_read",
                       [](const void* x, hipStream_t s) { auto& a = *(const KvCall*)x; return launch_kv_read(a.c, a.bt, a.k, a.v, s); },

@@ -45,8 +45,8 @@ class KvCache:
         import torch
 
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        if page_size <= 0 or page_size % 32:
-            raise InvalidArgument("page_size is a multiple of 32")
+        if page_size <= 0 or page_size % 32 or page_size > 1024:
+            raise InvalidArgument("page_size is a multiple of 32, at most 1024")
         pool = torch.empty(n_pages, kv_heads, page_size // 32, 34 * head_dim, dtype=torch.uint8, device=dev)
         bounds = torch.empty(n_pages, kv_heads, 2, head_dim, dtype=torch.int8, device=dev)
         self._take(pool, bounds, torch.empty(n_pages, kv_heads, dtype=torch.uint8, device=dev))
@@ -68,6 +68,8 @@ class KvCache:
             raise InvalidArgument("pool, bounds and bound_exps are of one cache")
         if size // 34 not in (64, 128, 256):
             raise InvalidVectorDimension("head_dim is 64, 128 or 256")
+        if not 0 < n <= 1 << 31 or not 0 < h <= 4096 or not 0 < tiles <= 32:
+            raise InvalidArgument("a cache has 1 .. 2^31 pages of at most 1024 tokens and 1 .. 4096 heads")
         for t, want in ((pool, torch.uint8), (bounds, torch.int8), (bound_exps, torch.uint8)):
             if t.dtype != want or not t.is_contiguous() or t.device != pool.device:
                 raise InvalidArgument("the cache's buffers are contiguous uint8, int8 and uint8 tensors of one device")

@@ -589,11 +589,12 @@ typedef struct gvdb_kv_rows {
 /* Quantises rows k and v into tokens lengths[s] .. of each sequence and makes
  * the touched pages' bounds new over every token that they hold up to there.
  * Tokens behind stay what they were.  A page must not be written for two
- * sequences in one call. */
+ * sequences, or at two places of one, in one call (pages that are only read may
+ * be anywhere in the table, and more than once). */
 gvdb_status gvdb_kv_append_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
                                   const gvdb_kv_rows* v, void* stream);
 /* The stored values of the same tokens, rounded once to the rows' type.
- * k or v may be NULL. */
+ * k or v may be NULL.  Output rows and heads must not overlap. */
 gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
                                 const gvdb_kv_rows* v, void* stream);
 /* Scratch of the attention calls (top: 0 for gvdb_kv_attend_device). */
@@ -604,7 +605,8 @@ gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batc
  * length - n + i + 1 of its length tokens, else all of them.  Query head h
  * reads key/value head h / (q_heads / kv_heads).  A row that sees no token is 0
  * (lse: -inf).  lse: device [rows][q_heads] f32, the natural logarithm of the
- * softmax's denominator, or NULL.  q and out: one type, q_heads heads.  Sums and
+ * softmax's denominator, or NULL.  q and out: one type, q_heads heads; out's rows must not overlap, and out may
+ * be q itself.  A row of q that is not finite spoils no other row.  Sums and
  * statistics are kept in 32 bits; keys, values and queries enter the products
  * exactly, the probabilities in 16 bits for bf16 and f16 rows (in 8 where bf16
  * rows come to 128 and more a sequence, a group's heads counted) and in 24 for

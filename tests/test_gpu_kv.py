@@ -415,6 +415,26 @@ def test_strided_misaligned_and_given_outputs(kv):
         assert (got[7:] == 0).all() and (chosen[7:] == -1).all()
 
 
+@pytest.mark.parametrize("dtype,new,lens", [("bf16", (2, 2), (9000, 4001)), ("f32", (3, 1), (5000, 2222)), ("f16", (90, 70), (3000, 700)),
+                                            ("bf16", (5, 0), (7, 640))])
+def test_hints_decide_nothing(kv, dtype, new, lens):
+    """Hints far below and above the truth, with and without `cu`; and the queries' own memory for the output."""
+    st = Store(kv, 40, dtype, 2, 64, 32, lens)
+    q = queries(41, dtype, new, 4, 64).cuda()
+    cu = i32(np.cumsum((0,) + new).tolist())
+    for hints in ({"max_new": 1, "max_len": 1}, {"max_new": 3, "max_len": 100}, {"max_new": 4000000000, "max_len": 4000000000}):
+        lse = torch.empty(q.shape[:2], device="cuda")
+        check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), cu=cu, lse=lse, **hints), lse)
+        if new[0] == new[1]:
+            check_attend(st, q, new, st.cache.attend(q, st.table, st.lengths(), **hints))
+    for cus in [cu] + [None] * (new[0] == new[1]):
+        want, own = st.cache.attend(q, st.table, st.lengths(), cu=cus), q.clone()
+        assert st.cache.attend(own, st.table, st.lengths(), cu=cus, out=own) is own and torch.equal(own, want)
+        (want, pages), own = st.cache.attend_topk(q, st.table, st.lengths(), 5, cu=cus), q.clone()
+        _, again = st.cache.attend_topk(own, st.table, st.lengths(), 5, cu=cus, out=own)
+        assert torch.equal(own, want) and torch.equal(again, pages)
+
+
 # ---- attention over chosen pages --------------------------------------------------------------
 @pytest.mark.parametrize("dtype,Hq,heads,D,page,lens,new,top,first,recent", [
     ("bf16", 8, 2, 128, 64, (5000,), (1,), 8, 1, 1),
@@ -478,6 +498,24 @@ def test_topk_of_long_tables(kv, pages, new):
         want = plain.choose(q[i].double().cpu().numpy(), [fifty[j] for j in order], seen, top, 1, 2)
         assert got[i, 0].tolist() == want
     check_attend(long, q, (new,), out, chosen=got)
+
+
+def test_topk_by_a_full_lds(kv):
+    """Hints decide where scores lie, not what is chosen: a table whose scores fill a workgroup's LDS, and the same by way of memory."""
+    D, page, top, pages = 64, 32, 9, 15000
+    rng = np.random.default_rng(33)
+    st = Store(kv, 34, "bf16", 1, D, page, (page * 50,))
+    order = rng.integers(0, 50, pages)
+    table = st.table[:, torch.from_numpy(order).cuda()].contiguous()
+    length = pages * page - 5
+    for new in (1, 2):
+        q = queries(35, "bf16", (new,), 3, D).cuda()
+        _, chosen = st.cache.attend_topk(q, table, i32([length]), top, max_len=1)
+        fifty = st.bounds(0, 0)
+        for i in range(new):
+            seen = (length - new + i) // page + 1
+            assert chosen[i, 0].tolist() == plain.choose(q[i].double().cpu().numpy(), [fifty[j] for j in order], seen, top, 1, 1)
+        assert torch.equal(chosen, st.cache.attend_topk(q, table, i32([length]), top)[1])
 
 
 def test_topk_ties_take_the_lowest_page(kv):
@@ -617,7 +655,8 @@ def test_python_refusals(kv):
                 lambda: c.attend(q, t, n, lse=torch.zeros(2, 3, device="cuda")), lambda: c.attend_topk(q, t, n, 0),
                 lambda: c.attend_topk(q, t, n, 2, first=2, recent=1), lambda: c.append(q[:, :2], q, t, n),
                 lambda: c.append(q[:, :2], q[:, :2].float(), t, n), lambda: c.attend(q, t.t(), n),
-                lambda: kv.KvCache(4, 2, 96), lambda: kv.KvCache.from_buffers(c.pool, c.bounds[:1], c.bound_exps)):
+                lambda: kv.KvCache(4, 2, 96), lambda: kv.KvCache(4, 2, 64, 2048), lambda: kv.KvCache(0, 2, 64), lambda: kv.KvCache(4, 5000, 64),
+                lambda: c.attend(q, t, n, out=q[:1].expand(2, 4, 64)), lambda: c.read(t, n, 2, out=(q[:, :1].expand(2, 2, 64), q[:, :2])), lambda: kv.KvCache.from_buffers(c.pool, c.bounds[:1], c.bound_exps)):
         with pytest.raises((InvalidArgument, Exception)) as e:
             bad()
         assert "VectorDbError" in [k.__name__ for k in type(e.value).__mro__], e.value

@@ -113,6 +113,17 @@ def test_row_refusals(call):
     assert call.L.gvdb_kv_read_device(C.byref(call.cache), C.byref(call.batch), C.byref(call.rows), C.byref(v), None) == ARG
 
 
+@pytest.mark.parametrize("field,value", [("row_stride", 0), ("row_stride", 127), ("row_stride", -127), ("head_stride", 0), ("head_stride", 64)])
+def test_outputs_do_not_overlap(call, field, value):
+    setattr(call.out, field, value)
+    assert call.attend() == ARG and "overlapping" in call.why()
+    assert call.topk() == ARG and "overlapping" in call.why()
+    setattr(call.rows, field, value)
+    for k, v in ((call.rows, None), (None, call.rows)):
+        rc = call.L.gvdb_kv_read_device(C.byref(call.cache), C.byref(call.batch), k and C.byref(k), v and C.byref(v), None)
+        assert rc == ARG and "overlapping" in call.why()
+
+
 def test_attention_refusals(call):
     assert call.attend(heads=5) == ARG
     assert call.attend(heads=0) == ARG
