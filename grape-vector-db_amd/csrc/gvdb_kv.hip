@@ -1540,12 +1540,12 @@ __device__ __forceinline__ void score_pages(const u4 (&pb)[D / 32], uint32_t e, 
     for (int r = 0; r < 4; ++r) best[r] = be[r] == 255u ? 3.402823466e38f : best[r];
 }
 
-// Scores of pages [from, to) for CG times 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256:
-// half of them); `put` takes four neighbouring pages' scores for the g-th 16 columns.
+// Scores of pages [from, to) for CG times 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256, and
+// several times 16 columns: half of them, by half the code); `put` takes four neighbouring pages' scores for the g-th 16 columns.
 template <int D, int CG, class Put>
 __device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt, uint32_t b, uint32_t h, const ScoreCols<D> (&col)[CG],
                                             uint32_t width, int64_t from, int64_t to, uint32_t wave, uint32_t waves, uint32_t lane, Put put) {
-    constexpr int NB = D == 256 ? 2 : 4;
+    constexpr int NB = D == 256 || CG > 1 ? 2 : 4;
     const uint32_t q4 = lane >> 4, n16 = lane & 15u;
     auto look = [&](int64_t p) { return p + lane < to ? (int)page_of(c, bt, b, (uint32_t)(p + lane)) : -1; };
     int64_t p = from + wave * 64;
@@ -1553,7 +1553,7 @@ __device__ __forceinline__ void score_range(const KvCache& c, const KvBatch& bt,
     for (; p < to; p += waves * 64) {
         const uint32_t e = page >= 0 ? c.bound_exps[(uint64_t)page * c.heads + h] : 255u;
         const int now = page;
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < 4; s += NB) {
             if (p + 16 * s >= to) break;
             u4 pb[NB][D / 32];
@@ -1703,12 +1703,23 @@ __device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uin
 }
 
 // One workgroup: the pages of `per` tokens of a sequence (at most CG times 16 / width) and one key head, scored into LDS and chosen
-// there.  The tokens share the bounds that it reads, 2 D + 1 bytes a page; 384 tokens over 1024 pages take 67 us one sixteen
-// columns a workgroup.
+// there.  The tokens share the bounds that it reads, 2 D + 1 bytes a page.  CG > 1: a wave quantises sixteen columns for all of them,
+// and hands them on through LDS; with every wave at all of them, and the loop over pages unrolled, it waited for its own code.
+// 384 tokens, 4 heads, 1024 pages: 37 us (45 before; 67 by one sixteen columns a workgroup), about a third each for the prologue, the
+// scores and the choice, none of them near a rate of the card: 192 workgroups, a chain of short phases.
 template <int D, int T, int CG>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t per) {
     extern __shared__ float s_sc[];  // [per][table_width]
-    __shared__ ChooseLds s_choose;
+    // columns, each wave's sixteen for all the waves; then the choice
+    struct Cols {
+        u4 x[D / 32][64];
+        uint32_t e[64];
+    };
+    __shared__ union Lds {
+        ChooseLds choose;
+        Cols col[CG];
+    } s_lds;
+    ChooseLds& s_choose = s_lds.choose;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t q4 = lane >> 4, n16 = lane & 15u;
     const uint32_t h = blockIdx.x % c.heads, unit = blockIdx.x / c.heads, b = unit / tok_tiles;
@@ -1724,11 +1735,29 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
             for (uint32_t g0 = 0; g0 < group; g0 += width) {
                 const uint32_t gh = g0 + n16 % width;
                 ScoreCols<D> col[CG];
-#pragma unroll
-                for (int g = 0; g < CG; ++g) {
+                auto take = [&](int g, ScoreCols<D>& x) {
                     const int tok = g * (int)toks16 + (int)my;
-                    col[g].template load<T>(a, tok < toks && gh < group,
-                                            (int64_t)(r0 + t0 + tok) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+                    x.template load<T>(a, tok < toks && gh < group,
+                                       (int64_t)(r0 + t0 + tok) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+                };
+                if constexpr (CG == 1) {
+                    take(0, col[0]);
+                } else {
+                    if (g0) __syncthreads();
+                    if (wave < CG) {
+                        take((int)wave, col[0]);
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k) s_lds.col[wave].x[k][lane] = col[0].pos[k], s_lds.col[wave].x[D / 64 + k][lane] = col[0].neg[k];
+                        s_lds.col[wave].e[lane] = col[0].e | (col[0].on ? 256u : 0u);
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int g = 0; g < CG; ++g) {
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k) col[g].pos[k] = s_lds.col[g].x[k][lane], col[g].neg[k] = s_lds.col[g].x[D / 64 + k][lane];
+                        const uint32_t e = s_lds.col[g].e[lane];
+                        col[g].e = e & 255u, col[g].on = e > 255u;
+                    }
                 }
                 score_range<D, CG>(c, bt, b, h, col, width, 0, seen, wave, kChooseWaves, lane, [&](int g, int64_t p, const float(&best)[4]) {
                     const int tok = g * (int)toks16 + (int)my;
