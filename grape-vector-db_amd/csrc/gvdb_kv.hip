@@ -1650,30 +1650,34 @@ __device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uin
     uint32_t over;
     if (want > 0 && want <= W * 64) (void)halve(maxima, W * 64, want, 2 * W, floor, hi + 1, over, lane);
     // the list of what is left; where it is too long, the pages themselves are gone over
-    uint32_t mine = 0;
-#pragma unroll 2
-    for (uint32_t j = j0; j < j1; j += 64) mine += (uint32_t)__popcll(__ballot(j + lane < j1 && f32_order(sc(min(j + lane, j1 - 1))) >= floor));
-    if (lane == 0) s.count[wave] = mine;
-    meet();
     uint32_t at = 0, n = 0;
+    if constexpr (W > 1) {  // each wave's pages go behind those of the waves before
+        uint32_t mine = 0;
+#pragma unroll 2
+        for (uint32_t j = j0; j < j1; j += 64) mine += (uint32_t)__popcll(__ballot(j + lane < j1 && f32_order(sc(min(j + lane, j1 - 1))) >= floor));
+        if (lane == 0) s.count[wave] = mine;
+        meet();
 #pragma unroll
-    for (uint32_t w = 0; w < W; ++w) {
-        const uint32_t x = s.count[W > 1 ? w : wave];
-        if (w < part) at += x;
-        n += x;
+        for (uint32_t w = 0; w < W; ++w) {
+            const uint32_t x = s.count[w];
+            if (w < part) at += x;
+            n += x;
+        }
     }
-    const bool listed = n <= kCap;
-    if (listed) {
-#pragma unroll 1
+    if (n <= kCap) {
+#pragma unroll 2
         for (uint32_t j = j0; j < j1; j += 64) {
-            const uint32_t k = j + lane < j1 ? f32_order(sc(j + lane)) : 0u;
+            const uint32_t k = f32_order(sc(min(j + lane, j1 - 1)));
             const bool in = j + lane < j1 && k >= floor;
             const uint64_t m = __ballot(in);
+            if (!m) continue;
             const uint32_t to = at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
-            if (in) list_key[to] = k, list_page[to] = j + lane;
+            if (in && to < kCap) list_key[to] = k, list_page[to] = j + lane;
             at += (uint32_t)__popcll(m);
         }
     }
+    if constexpr (W == 1) n = at;
+    const bool listed = n <= kCap;
     meet();
     if (W == 1 || wave == 0) {
         for (uint32_t i = lane; i < a.first; i += 64) out[i] = (int32_t)i;
@@ -1705,8 +1709,8 @@ __device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uin
 // One workgroup: the pages of `per` tokens of a sequence (at most CG times 16 / width) and one key head, scored into LDS and chosen
 // there.  The tokens share the bounds that it reads, 2 D + 1 bytes a page.  CG > 1: a wave quantises sixteen columns for all of them,
 // and hands them on through LDS; with every wave at all of them, and the loop over pages unrolled, it waited for its own code.
-// 384 tokens, 4 heads, 1024 pages: 37 us (45 before; 67 by one sixteen columns a workgroup), about a third each for the prologue, the
-// scores and the choice, none of them near a rate of the card: 192 workgroups, a chain of short phases.
+// 384 tokens, 4 heads, 1024 pages: 35 us (45 before; 67 by one sixteen columns a workgroup), about a third each for the prologue, the
+// scores and the choice, none of them near a rate of the card: 192 workgroups, a chain of short phases.  3800 pages: 95 us.
 template <int D, int T, int CG>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t per) {
     extern __shared__ float s_sc[];  // [per][table_width]
@@ -1776,7 +1780,10 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
             int32_t* out = a.chosen + ((uint64_t)(r0 + t0 + t) * c.heads + h) * a.top;
             const float* sc = s_sc + t * bt.table_width;
             // a page beyond the table is the last: it is among the recent ones, or scores as one that is not there
-            auto score = [=](uint32_t j) { return j < in_lds ? sc[j] : 3.402823466e38f; };
+            auto score = [=](uint32_t j) {
+                const float x = sc[min(j, in_lds - 1)];
+                return j < in_lds ? x : 3.402823466e38f;
+            };
             if (mine > (int64_t)a.top && toks == 1) {
                 choose_pages<kChooseWaves>(a, score, (uint32_t)mine, out, s_choose, wave, lane);
             } else if ((uint32_t)t % kChooseWaves == wave) {  // each wave its token
@@ -1840,7 +1847,11 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch
     }
     const float* sc = a.scores + ((uint64_t)token * c.heads + h) * bt.table_width;
     const uint32_t width = bt.table_width;
-    choose_pages<kChooseWaves>(a, [=](uint32_t j) { return j < width ? sc[j] : 3.402823466e38f; }, (uint32_t)seen, out, s_choose,
+    auto score = [=](uint32_t j) {
+        const float x = sc[min(j, width - 1)];
+        return j < width ? x : 3.402823466e38f;
+    };
+    choose_pages<kChooseWaves>(a, score, (uint32_t)seen, out, s_choose,
                                __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63u);
 }
 
@@ -1947,13 +1958,16 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
         return hipErrorInvalidValue;
     if (fused) {
         const uint32_t lds = per * bt.table_width * 4;
-        if (many) {
-            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_choose<D, T, D == 256 ? 2 : 4>
+        auto launch = [&](auto cg) {
+            constexpr int CG = decltype(cg)::value;
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_choose<D, T, D == 256 && CG == 4 ? 2 : CG>
                                            <<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
-        } else {
-            KV_DISPATCH(c.dim, a.q.dtype,
-                        (k_kv_choose<D, T, 1><<<(uint32_t)(others * tok_tiles), kChooseThreads, lds, s>>>(c, bt, a, tok_tiles, per)));
-        }
+        };
+        // as many times 16 columns as the workgroup's tokens take: half the table's tokens fit LDS where it has 3800 pages, and the other
+        // half's columns would cost as much (384 tokens, 4 heads: 149 us, so 115)
+        if (per <= per16) launch(Const<1>());
+        else if (per <= 2 * per16) launch(Const<2>());
+        else launch(Const<4>());
         GVDB_LAUNCH_CHECK();
     } else {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));
