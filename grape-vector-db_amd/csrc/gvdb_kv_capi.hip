@@ -127,15 +127,19 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     const uint64_t tiles = top ? (uint64_t)std::min(top, bt.table_width) * (c.page / 32) : ((uint64_t)bt.max_len + 31) / 32;
     const uint64_t rows_each = top ? group : bt.max_new * group;
     const uint64_t units0 = top ? bt.rows : bt.n_seqs;
+    // Workgroups that have rows, of `w` rows each: with `cu` the sequences are of several lengths, and `rows` says how many there are in all.
+    auto busy_of = [&](uint64_t w, uint64_t n_units) { return std::min(n_units, (bt.rows * group / w + bt.n_seqs) * c.heads); };
     // 128 rows and more share the values' expansion: a chunk of 2048 tokens takes 632 us so and 1110 us in tiles of 16 rows; at 64 rows
-    // a sequence 40 and 35 us, at 128 rows 49 and 50.  In 32 bits the pieces do not fit the registers: 130 and 117 us at 512 rows.
-    a.many = !top && dtype != GVDB_F32 && rows_each >= 128;
+    // a sequence 40 and 35 us, at 128 rows 49 and 50.  It wants three quarters of a workgroup a CU, parts of 512 tokens counted: 24 chunks
+    // of 64 tokens over 250 take 19 us so and 28 in tiles of 16 rows, 16 of them over 900 36 and 32, one of 512 over 2000 28 and 26, over
+    // 16000 33 and 37.  In 32 bits the pieces do not fit the registers: 130 and 117 us at 512 rows.
+    const uint64_t busy128 = busy_of(128, units0 * c.heads * ((rows_each + 127) / 128));
+    a.many = !top && dtype != GVDB_F32 && rows_each >= 128 && busy128 * (tiles > 32 ? tiles : 16) >= 16 * 192;
     uint64_t row_tiles = a.many ? (rows_each + 127) / 128 : (rows_each + 15) / 16;
     // grids stay below 2^20 tiles of rows where the hints are loose: the kernels stride over the rest
     row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
     const uint64_t units = units0 * c.heads * row_tiles;
-    // workgroups that have rows: with `cu` the sequences are of several lengths, and `rows` says how many there are in all
-    const uint64_t busy = top ? units : std::min(units, (bt.rows * group / (a.many ? 128 : 16) + bt.n_seqs) * c.heads);
+    const uint64_t busy = top ? units : busy_of(a.many ? 128 : 16, units);
     // Two workgroups a CU: four waves a SIMD pair read 5.3 TB/s.  64 sequences of up to 10000 tokens: 65 us with one, 58 with
     // two, 69 with three, 65 with four; 4 x 256K tokens: 263, 215, 231, 226 us.
     const uint64_t slots = 512;

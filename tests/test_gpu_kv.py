@@ -353,6 +353,71 @@ def test_attend_many_rows(kv, dtype, Hq, heads, D, page, lens, new, causal):
     check_attend(st, q, new, out, lse, causal=causal)
 
 
+def crowd(st, q, new, copies, lse=None, **more):
+    """The same sequences many times over, as many as take whole workgroups of rows: every copy's output is the first's."""
+    rows = len(q)
+    many = torch.empty(rows * copies, q.shape[1], device="cuda")
+    out = st.cache.attend(q.repeat(copies, 1, 1), st.table.repeat(copies, 1), st.lengths().repeat(copies),
+                          cu=i32(np.cumsum((0,) + tuple(new) * copies).tolist()), lse=many, max_new=max(new), **more)
+    bits = out.view(torch.int16 if out.element_size() == 2 else torch.int32).view(copies, rows, *q.shape[1:])
+    assert torch.equal(bits, bits[:1].expand_as(bits))
+    if lse is not None:
+        lse.copy_(many[:rows])
+    return out[:rows]
+
+
+@pytest.mark.parametrize("dtype,Hq,heads,D,page,lens,new,causal,copies", [
+    ("bf16", 8, 2, 64, 32, (400, 70, 9), (33, 70, 40), True, 60),     # the last sequence is shorter than its rows
+    ("f16", 8, 2, 64, 32, (130, 77), (64, 40), False, 60),
+    ("f16", 8, 2, 128, 64, (500, 0), (200, 3), False, 30),
+    ("bf16", 6, 2, 128, 64, (333,), (90,), True, 60),
+    ("bf16", 4, 2, 256, 64, (300,), (129,), True, 64),
+    ("f16", 3, 1, 256, 1024, (1000,), (47,), True, 128),
+])
+def test_attend_crowds_of_rows(kv, dtype, Hq, heads, D, page, lens, new, causal, copies):
+    st = Store(kv, 45, dtype, heads, D, page, lens)
+    q = queries(46, dtype, new, Hq, D).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    check_attend(st, q, new, crowd(st, q, new, copies, lse, causal=causal, max_len=max(lens)), lse, causal=causal)
+
+
+@pytest.mark.parametrize("dtype,Hq,heads,D,lens,new", [("bf16", 64, 1, 64, (4000,), (5,)), ("f16", 32, 2, 128, (3000, 2500), (8, 9)),
+                                                       ("bf16", 16, 1, 256, (1500,), (9,))])
+def test_attend_many_rows_in_parts(kv, dtype, Hq, heads, D, lens, new):
+    """A table far wider than the sequences: parts are cut for the width, and most of them hold nothing."""
+    st = Store(kv, 47, dtype, heads, D, 64, lens, width=2000)
+    q = queries(48, dtype, new, Hq, D).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), cu=i32(np.cumsum((0,) + new).tolist()), lse=lse, max_new=max(new))
+    check_attend(st, q, new, out, lse)
+
+
+@pytest.mark.parametrize("dtype,Hq,D,page", [("bf16", 2, 128, 64), ("f16", 2, 64, 32), ("bf16", 2, 256, 96), ("f16", 4, 128, 32)])
+def test_what_is_masked_in_a_crowd_may_hold_anything(kv, dtype, Hq, D, page):
+    for poison in (float("nan"), float("inf"), -float("inf")):
+        st = Store(kv, 49, dtype, 1, D, page, (150,))
+        k = torch.from_numpy(np.random.default_rng(1).standard_normal((4, 1, D))).to(DT[dtype]).cuda()
+        v = k.clone()
+        v[1, :, 40] = poison   # token 121: a value, channels 32 .. 63
+        k[3, :, 7] = poison    # token 123: a key
+        st.cache.append(k, v, st.table, i32([120]))
+        st.k[0][120:124], st.v[0][120:124] = plain.stored(k.double().cpu().numpy()), plain.stored(v.double().cpu().numpy())
+        q = queries(50, dtype, (150,), Hq, D).cuda()
+        q[5, 1, 0] = poison
+        out = crowd(st, q, (150,), 96, max_len=150)
+        want = np.zeros((150, Hq, D), bool)
+        want[121:, :, 32:64] = True
+        want[123:] = True
+        want[5, 1] = True
+        assert np.array_equal(torch.isnan(out).cpu().numpy(), want)
+        check_attend(st, q, (150,), out, skip={(r, h) for r in range(121, 150) for h in range(Hq)} | {(5, 1)})
+        table = st.table.clone()
+        table[0, 1] = -1       # a page that is not there
+        st.table = table
+        nan = torch.isnan(crowd(st, q, (150,), 96, max_len=150)).flatten(1).all(1)
+        assert nan.tolist() == [r >= page for r in range(150)]
+
+
 def test_rows_outside_every_sequence(kv):
     """cu may begin behind the first row and end before the last: those rows are left alone, or 0 where the call makes the output."""
     D, Hq, heads = 64, 4, 2
