@@ -929,8 +929,8 @@ __device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j,
 // turn, one step's loads in flight while another is worked on, and join their parts through LDS.  With one query token a
 // sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it.
 template <int D, int T, bool CHOSEN>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
-    constexpr int NP = pieces(T), NT = kStep<D, NP>;
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 : 3) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
+    constexpr int NP = pieces(T), NT = 1;
     __shared__ JoinLds<D> s;
     clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

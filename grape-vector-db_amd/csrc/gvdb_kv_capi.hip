@@ -143,27 +143,35 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     // Two workgroups a CU: four waves a SIMD pair read 5.3 TB/s.  64 sequences of up to 10000 tokens: 65 us with one, 58 with
     // two, 69 with three, 65 with four; 4 x 256K tokens: 263, 215, 231, 226 us.
     const uint64_t slots = 512;
-    // The line helps while sequences are of several lengths (250 of them, 8 heads: 94 us, whole units 102); chosen pages are of one
-    // length, and whole units win from 1024 on (384 tokens, 4 heads: 100 us, the line 103).
-    const uint64_t line_most = (top ? 2 : 8) * slots;
+    // Whole, a unit of 16 rows takes 6 us and 0.17 a tile; shared, all of them 14 us (the join's launch among it) and their share of the
+    // card.  Units of one length (chosen pages, one sequence's rows) are shared while few and long: 8 units of 47 tiles 15 us and 14 whole,
+    // of 125 15 and 27, 128 of 125 27 and 28, 256 of 188 53 and 48, 192 of 128 chosen 52 and 50.  Sequences of several lengths leave
+    // a card of whole units uneven: 512 of up to 63 tiles 25 us and 20 whole, of up to 188 40 and 47, 2000 of up to 125 94 and 91, of up
+    // to 313 188 and 209.
+    const bool shared = a.many ? busy < 2 * slots && tiles > 32
+                        : top || bt.n_seqs == 1 ? units < 200 && tiles * (200 - units) > 9000
+                                                : tiles > 48 + units / 8;
     a.row_tiles = (uint32_t)row_tiles;
     a.splits = 1;
     a.chunk = (uint32_t)(tiles + 1) / 2 * 2;
-    if (a.many ? busy < 2 * slots && tiles > 32 : tiles > 32 && units < line_most) {  // else a workgroup takes its rows' tiles whole
+    if (shared) {
         const uint64_t line = units0 * ((rows_each + 15) / 16);
         const uint64_t most = line * (top ? (uint64_t)top : (uint64_t)bt.table_width + 1) * (c.page / 32);
         if (!a.many && (top || !bt.cu) && line <= kMaxUnits && most < (1ull << 31)) {
-            // the rows of a unit are known: every wave gets the same share of all tiles, of 4 at least
+            // the rows of a unit are known: every wave gets the same share of all tiles, of 4 at least; of long sequences more, for the
+            // join's sake, as below (8 heads, one sequence of 125 tiles: 13 us by 4, 16 by 8; of 938 26 and 21)
             a.units = (uint32_t)line;
             a.lanes = (uint32_t)std::max<uint64_t>(1, slots / c.heads) * 4;
-            a.least = 4;
+            a.least = std::max<uint32_t>(4, (uint32_t)std::sqrt((double)tiles) / 4);
             a.slot_rows = (uint32_t)std::min<uint64_t>(16, rows_each);
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
         } else {
             // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 336 us,
-            // for 1024 of them 354, for 512 432), or 768 of 16 rows (up to 5 tokens of 8 sequences over 20000: 37 us, for 512 47)
-            const uint64_t parts = a.many ? 4 * slots : slots + slots / 2;
-            a.chunk = (uint32_t)std::max<uint64_t>(a.many ? 16 : 8, ((busy * tiles + parts - 1) / parts + 1) / 2 * 2);  // whole steps
+            // for 1024 of them 354, for 512 432), or 3072 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
+            // 768 121).  Of 16 tiles at least, for 128 rows; of 16 rows a part's time grows with its tiles and the join's with the parts,
+            // so of the square root of all tiles (best of 6 .. 32: 94 tiles 8 to 12, 250 12 to 16, 625 24, 938 32)
+            const uint64_t parts = a.many ? 2048 : 3072, least = a.many ? 16 : std::max<uint64_t>(8, (uint64_t)std::sqrt((double)tiles));
+            a.chunk = (uint32_t)((std::max(least, (busy * tiles + parts - 1) / parts) + 1) / 2 * 2);  // whole steps
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         }
     }

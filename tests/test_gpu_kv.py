@@ -583,6 +583,20 @@ def test_topk_by_a_full_lds(kv):
         assert torch.equal(chosen, st.cache.attend_topk(q, table, i32([length]), top)[1])
 
 
+@pytest.mark.parametrize("dtype,Hq,heads,D,lens,new,top", [
+    ("f16", 8, 2, 64, (4000, 3500), (1, 1), 60), ("f32", 4, 2, 128, (2500, 2900, 17), (2, 2, 2), 50), ("bf16", 6, 3, 256, (3000, 2222), (1, 1), 48),
+    ("f32", 5, 1, 256, (2600,), (3,), 47), ("bf16", 36, 2, 128, (1900, 2000, 2600), (2, 2, 2), 46), ("f32", 3, 1, 64, (40, 3300), (1, 1), 47)])
+def test_few_rows_share_the_card(kv, dtype, Hq, heads, D, lens, new, top):
+    """Few rows of many tokens or pages, in equal shares of all tiles; more rows a head than 16 among them."""
+    st = Store(kv, 51, dtype, heads, D, 64, lens)
+    q = queries(52, dtype, new, Hq, D).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = st.cache.attend(q, st.table, st.lengths(), lse=lse)
+    check_attend(st, q, new, out, lse)
+    out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), top, lse=lse)
+    check_attend(st, q, new, out, lse, chosen=chosen.cpu().numpy())
+
+
 def test_topk_ties_take_the_lowest_page(kv):
     """Equal pages score alike: the lowest of them are taken; all-zero queries and keys too."""
     D, page = 64, 32
