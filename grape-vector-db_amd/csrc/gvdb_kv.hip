@@ -577,11 +577,6 @@ struct Rows {
     float m, l;         // largest exponent (base 2) of the row; this lane's share of the sum
 };
 
-// Tiles that a wave works on at a time: two, where the registers hold two and the two whose loads are in flight at two
-// waves a SIMD.  One maximum, one look at what is odd and one change of scale a step instead of a tile.
-template <int D, int NP>
-constexpr int kStep = D == 256 || NP == 3 ? 1 : 2;
-
 // Scores of a tile: s[i][r] of token 8q + 2r + i, without the scale.
 template <int D, int NP>
 __device__ __forceinline__ void tile_scores(const Rows<D, NP>& w, const Tile<D>& t, f4 (&s)[2]) {
@@ -679,37 +674,28 @@ __device__ __forceinline__ void tile_values(Rows<D, NP>& w, const Tile<D>& t, co
     }
 }
 
-template <int D, int NT>
-struct Step {  // tiles whose loads were issued together
-    Tile<D> t[NT];
-    bool there[NT];
-    int32_t base[NT];  // first tokens
+template <int D>
+struct Step {  // a tile whose loads were issued
+    Tile<D> t;
+    bool there;
+    int32_t base;  // its first token
 };
 
-// One step for 16 rows: the running maximum and sum of a softmax over its NT * 32 tokens.
-template <int D, int NP, bool CHOSEN, int NT>
-__device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const Job<CHOSEN>& j, float c2, uint32_t lane) {
+// One step for 16 rows: the running maximum and sum of a softmax over its 32 tokens.  With two tiles a step, one maximum and one look at
+// what is odd serve both, but a wave's first product waits for twice the loads, and its registers leave room for two waves a SIMD: 64
+// sequences of 1500 tokens take 26 us so, 22 tile by tile; 4 of 262144 215 and 205.
+template <int D, int NP, bool CHOSEN>
+__device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D>& st, const Job<CHOSEN>& j, float c2, uint32_t lane) {
     constexpr int PP = NP < 2 ? 2 : NP;  // of a probability: with one, half of a bf16 row's error would be the probabilities'
-    f4 s[NT][2];
-    uint32_t odd = 0;
-    bool plain = true;
+    f4 s[2];
+    tile_scores<D, NP>(w, st.t, s);
+    const bool plain = st.there && (int64_t)st.base + 32 <= j.least;
+    if (!plain || __ballot(odd_scales(st.t) != 0)) settle_tile<D, NP>(w, st.t, s, j, st.there, st.base, lane);
+    float top = s[0][0];
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        tile_scores<D, NP>(w, st.t[x], s[x]);
-        odd |= odd_scales(st.t[x]);
-        plain &= st.there[x] && (int64_t)st.base[x] + 32 <= j.least;
-    }
-    if (!plain || __ballot(odd != 0)) {
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int x = 0; x < NT; ++x) settle_tile<D, NP>(w, st.t[x], s[x], j, st.there[x], st.base[x], lane);
-    }
-    float top = s[0][0][0];
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[x][i][e]);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
     top = row_max(top) * c2;
     const bool over = top > w.m + kSlack;
     top = over ? top : w.m;
@@ -722,21 +708,18 @@ __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D, NT>& st, const
 #pragma unroll
             for (int e = 0; e < 4; ++e) w.o[k][e] *= a;
     }
+    u4 pf[PP];
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-        u4 pf[PP];
+    for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][e], c2, -top));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][e], c2, -top));
+        uint32_t pc[PP];
+        pack_pieces<PP>(p0, p1, pc);
+        w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][0][e], c2, -top));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][1][e], c2, -top));
-            uint32_t pc[PP];
-            pack_pieces<PP>(p0, p1, pc);
-            w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
-#pragma unroll
-            for (int p = 0; p < PP; ++p) pf[p][e] = pc[p];
-        }
-        tile_values<D, NP, PP>(w, st.t[x], pf);
+        for (int p = 0; p < PP; ++p) pf[p][e] = pc[p];
     }
+    tile_values<D, NP, PP>(w, st.t, pf);
 }
 
 // Where a wave's next 64 tiles lie: lane i keeps the i-th of them, so that no tile's loads wait for the page table.
@@ -759,16 +742,13 @@ struct Feed {
         const uint64_t u = ((uint64_t)page * c.heads + h) * per_page + sub;
         lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
     }
-    // The loads of the step whose first tile is the i-th.  A tile that is not there is read as the pool's first, and not used.
-    template <int D, int NT>
-    __device__ __forceinline__ void load(const KvCache& c, uint32_t i, uint32_t lane, Step<D, NT>& st) const {
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            const uint32_t l = __builtin_amdgcn_readlane(lo, i + x), u = __builtin_amdgcn_readlane(hi, i + x);
-            st.there[x] = u != ~0u;
-            st.base[x] = (int32_t)__builtin_amdgcn_readlane((uint32_t)pos, i + x);
-            load_tile<D>(c.pool + (st.there[x] ? (uint64_t)u << 32 | l : 0) * (uint64_t)(34 * D), lane, st.t[x]);
-        }
+    // The loads of the i-th.  A tile that is not there is read as the pool's first, and not used.
+    template <int D>
+    __device__ __forceinline__ void load(const KvCache& c, uint32_t i, uint32_t lane, Step<D>& st) const {
+        const uint32_t l = __builtin_amdgcn_readlane(lo, i), u = __builtin_amdgcn_readlane(hi, i);
+        st.there = u != ~0u;
+        st.base = (int32_t)__builtin_amdgcn_readlane((uint32_t)pos, i);
+        load_tile<D>(c.pool + (st.there ? (uint64_t)u << 32 | l : 0) * (uint64_t)(34 * D), lane, st.t);
     }
 };
 
@@ -930,7 +910,7 @@ __device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j,
 // sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 : 3) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
-    constexpr int NP = pieces(T), NT = 1;
+    constexpr int NP = pieces(T);
     __shared__ JoinLds<D> s;
     clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -939,9 +919,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
     for (uint32_t row_tile = rest % a.row_tiles;; row_tile += a.row_tiles) {
         Job<CHOSEN> j;
         if (!j.set(c, bt, a, rest / a.row_tiles, row_tile, h, lane & 15u) || j.first >= j.rows) return;
-        const uint32_t steps = (j.tiles(c, bt, a) + NT - 1) / NT, chunk = a.chunk / NT;
-        const uint32_t s0 = (uint32_t)min((uint64_t)split * chunk, (uint64_t)steps);
-        const uint32_t s1 = split + 1 == a.splits ? steps : min(s0 + chunk, steps);
+        const uint32_t tiles = j.tiles(c, bt, a), s0 = (uint32_t)min((uint64_t)split * a.chunk, (uint64_t)tiles);
+        const uint32_t s1 = split + 1 == a.splits ? tiles : min(s0 + a.chunk, tiles);
         if (a.splits > 1 && s0 >= s1) continue;  // no part: k_kv_combine does not read it
         Rows<D, NP> w;
         clear(w);
@@ -950,11 +929,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
         const uint32_t mine = s0 + wave < s1 ? (s1 - s0 - wave + 3) / 4 : 0;
         const int32_t* list = j.list(c, a);
         Feed<CHOSEN> feed;
-        Step<D, NT> st, next;
+        Step<D> st, next;
         auto fill = [&](uint32_t it) {
-            const uint32_t step = s0 + wave + 4 * (it + lane / NT);
+            const uint32_t tile = s0 + wave + 4 * (it + lane);
             feed.none();
-            if (step < s1) feed.take(c, bt, j.b, h, list, a.top, step * NT + lane % NT);
+            if (tile < s1) feed.take(c, bt, j.b, h, list, a.top, tile);
         };
         if (mine) {
             fill(0);
@@ -964,9 +943,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
         for (uint32_t it = 0; it < mine; ++it) {
             st = next;
             if (it + 1 < mine) {
-                const uint32_t i = (it + 1) % (64 / NT);
+                const uint32_t i = (it + 1) % 64;
                 if (i == 0) fill(it + 1);
-                feed.load(c, i * NT, lane, next);
+                feed.load(c, i, lane, next);
             }
             work_step<D, NP>(w, st, j, a.scale_log2, lane);
         }
@@ -981,7 +960,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
 // of units, the next unit's queries among them.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
-    constexpr int NP = pieces(T), NT = kStep<D, NP>;
+    constexpr int NP = pieces(T);
     __shared__ uint32_t s_wsum[4], s_pref[kMaxUnits + 1];
     clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -992,7 +971,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
         for (uint32_t u = u0; u < u1; ++u) {
             s_pref[u] = sum;
             Job<CHOSEN> j;
-            if (j.set(c, bt, a, u / a.row_tiles, u % a.row_tiles, h, 0)) sum += (j.tiles(c, bt, a) + NT - 1) / NT;
+            if (j.set(c, bt, a, u / a.row_tiles, u % a.row_tiles, h, 0)) sum += j.tiles(c, bt, a);
         }
         uint32_t total;
         const uint32_t before = block_scan_u32(sum, s_wsum, &total);
@@ -1002,7 +981,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
         if (blockIdx.x == 0)
             for (uint32_t u = threadIdx.x; u <= a.units; u += 256) a.prefix[u] = s_pref[u];
     }
-    const uint32_t total = s_pref[a.units], share = max(a.least / NT, (total + a.lanes - 1) / a.lanes);
+    const uint32_t total = s_pref[a.units], share = max(a.least, (total + a.lanes - 1) / a.lanes);
     const uint32_t at = (uint32_t)min((uint64_t)w_id * share, (uint64_t)total), end = min(at + share, total);
     if (at >= end) return;
     // the unit that holds a step of the line
@@ -1022,15 +1001,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
     raw.load(a, j, lane >> 4);
     Feed<CHOSEN> feed;
     auto fill = [&](uint32_t it) {
-        const uint32_t step = at + it + lane / NT;
+        const uint32_t tile = at + it + lane;
         feed.none();
-        if (step >= end) return;
-        const uint32_t v = unit_of(step);
+        if (tile >= end) return;
+        const uint32_t v = unit_of(tile);
         Job<CHOSEN> f;
         f.unit = (int)(v / a.row_tiles), f.h = h, f.b = (uint32_t)f.unit;
-        if (!CHOSEN || a.row_seq(bt, f.unit, f.b)) feed.take(c, bt, f.b, h, f.list(c, a), a.top, (step - s_pref[v]) * NT + lane % NT);
+        if (!CHOSEN || a.row_seq(bt, f.unit, f.b)) feed.take(c, bt, f.b, h, f.list(c, a), a.top, tile - s_pref[v]);
     };
-    Step<D, NT> st, next;
+    Step<D> st, next;
     fill(0);
     feed.load(c, 0, lane, next);
     Rows<D, NP> w;
@@ -1049,9 +1028,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
         for (; it < to - at; ++it) {
             st = next;
             if (it + 1 < mine) {
-                const uint32_t i = (it + 1) % (64 / NT);
+                const uint32_t i = (it + 1) % 64;
                 if (i == 0) fill(it + 1);
-                feed.load(c, i * NT, lane, next);
+                feed.load(c, i, lane, next);
             }
             work_step<D, NP>(w, st, j, a.scale_log2, lane);
         }
@@ -1403,7 +1382,7 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
         const uint32_t row = (CHOSEN ? 0u : (uint32_t)(token - r0)) * group + head % group;
         const uint32_t u = (CHOSEN ? (uint32_t)token : b) * a.row_tiles + row / 16;
         const uint32_t p0 = a.prefix[u], p1 = a.prefix[u + 1], total = a.prefix[a.units];
-        const uint32_t share = max(a.least / kStep<D, pieces(T)>, (total + a.lanes - 1) / a.lanes);
+        const uint32_t share = max(a.least, (total + a.lanes - 1) / a.lanes);
         const uint32_t w0 = p0 / share, w1 = p1 > p0 ? (p1 - 1) / share : w0;
         if (p1 > p0 && w0 == w1) return;  // one wave took it whole
         parts = p1 > p0 ? w1 - w0 + 1 : 0;
