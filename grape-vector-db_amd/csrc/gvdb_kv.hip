@@ -289,8 +289,9 @@ struct Raw8 {
 
 // ---- append -----------------------------------------------------------------------------
 // One workgroup a touched page, head and part (keys, values).  D / 8 threads take a token, eight channels each; four neighbours
-// share a scale.  Four passes' loads are in flight at once.  Bound by the reads of k and v where there are many tokens, and by
-// its chain of loads (length, page, rows) where there is one.
+// share a scale.  Four passes' loads are in flight at once.  Bound by the reads of k and v where there are many tokens (16384 tokens
+// of 8 heads of 128 channels, bf16: 25 us, 3.4 TB/s read and written), and by its chain of loads (length, page, rows and the codes
+// that the page's bounds go over) where there is one: 64 sequences' next tokens 8 us.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows k, KvRows v, uint32_t slots) {
     constexpr uint32_t TPT = D / 8;       // threads a token
@@ -411,7 +412,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows
 
 // ---- read -------------------------------------------------------------------------------
 // A thread takes eight channels of one token and head, keys and values; a workgroup several tokens of one head, whose codes lie
-// side by side.  Bound by what it writes.
+// side by side.  Bound by what it writes (the same 16384 tokens: 17.5 us, 4.9 TB/s).
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_read(KvCache c, KvBatch bt, KvRows k, KvRows v) {
     constexpr uint32_t TPT = D / 8;
@@ -907,7 +908,9 @@ __device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j,
 // ---- attend -----------------------------------------------------------------------------
 // A workgroup takes 16 query rows of a unit and key head and one split of its tiles; its four waves take steps of them in
 // turn, one step's loads in flight while another is worked on, and join their parts through LDS.  With one query token a
-// sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it.
+// sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it where there are many (32 sequences of 32 pages:
+// 18.5 us).  One sequence of 768 tokens takes 9 us, 4 of them before the first product (length, table, tiles, one behind the other).
+// 384 tokens' own 40 pages of 32, 4 heads: 47 us, 5.7 TB/s out of the caches and three quarters of the cycles in vector instructions.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 : 3) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T);
@@ -957,9 +960,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
 // and wave w of a head takes the w-th of equal shares of that line, whatever the sequences' lengths are.  A unit that one
 // wave takes whole is written at once; the others' parts go to slot w + u (w and u only ever grow along the line: no two
 // parts share one) and are joined by k_kv_combine.  Waves never wait for one another, and loads run on over the borders
-// of units, the next unit's queries among them.
+// of units, the next unit's queries among them.  Bound by the reads: 4 sequences of 262144 tokens, 8 heads of 128 channels, 205 us with
+// the join, 5.6 TB/s; 64 of up to 10000, 57 us, 4.1 TB/s, of which 5 are the join and 5 the way to the first product.
 template <int D, int T, bool CHOSEN>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T);
     __shared__ uint32_t s_wsum[4], s_pref[kMaxUnits + 1];
     clear_rest<D, T>(c, bt, a);
@@ -1049,6 +1053,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attend_line(KvCach
 // into LDS (two buffers, one barrier a step), as [8 tokens][channels][16 bytes], the operand as it is read.
 // A row of keys stands for token t(row) with bits 2 and 3 exchanged, so that S^T leaves a lane with eight neighbouring
 // tokens of its query row, which O^T = V^T P^T takes as they are.  Channel j of sixteenth l lies at row 16 j + l of V^T.
+// Bound by the vector instructions that expand keys and reckon probabilities: 2048 tokens of 2 sequences over 10000, 32 heads on 8 of
+// 128 channels, 630 us, 950 TFLOP/s; vector instructions issue in 64 % of the cycles, the matrix units are busy in 41 %, and two
+// workgroups a CU, all that the registers hold, overlap them no further.
 template <int D, int NP>
 struct Rows32 {
     u4 qf[NP][D / 16];  // query pieces: lane 32 i + n has row n, channels [i D/2, (i+1) D/2)
@@ -1362,7 +1369,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_atte
 // ---- combine ----------------------------------------------------------------------------
 // Joins a row's parts: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 8 lanes hold the channels.  FEW (parts of whole
 // rows, at most 16): each of a wave's 512 / D groups of lanes joins a row of its own.  Else the groups share one row and take
-// every so many-th part; the order of the sum is the lanes', alike on every run.
+// every so many-th part; the order of the sum is the lanes', alike on every run.  Bound by its chain of loads: 4 to 7 us.
 template <int D, int T, bool CHOSEN, bool FEW>
 __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr uint32_t L = D / 8, G = 64 / L;
@@ -1777,7 +1784,8 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
     }
 }
 
-// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds.
+// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds.  One token of 1024 pages,
+// 8 heads: 6.5 and 6.5 us, chains of loads; 32 tokens of up to 1563: 16 us, 3 TB/s of bounds, and 10.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t chunks) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -140,15 +140,17 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
     const uint64_t units = units0 * c.heads * row_tiles;
     const uint64_t busy = top ? units : busy_of(a.many ? 128 : 16, units);
-    // Two workgroups a CU: four waves a SIMD pair read 5.3 TB/s.  64 sequences of up to 10000 tokens: 65 us with one, 58 with
-    // two, 69 with three, 65 with four; 4 x 256K tokens: 263, 215, 231, 226 us.
-    const uint64_t slots = 512;
+    // As many workgroups as the card's registers hold at once: three a CU of 64 channels, two of 128, one of 256.  128 channels, 8 heads,
+    // 64 sequences of up to 10000 tokens: 64 us with one, 58 with two, 66 with four; 4 x 262144 tokens: 230, 204, 237 us; 256 channels,
+    // 4 heads, 64 sequences of up to 20000: 150 us with half a one, 96 with one, 102 with two; 64 channels, 8 heads: 66 us with two, 63
+    // with three.
+    const uint64_t slots = c.dim == 256 ? 256 : c.dim == 128 ? 512 : 768;
     // Whole, a unit of 16 rows takes 6 us and 0.17 a tile; shared, all of them 14 us (the join's launch among it) and their share of the
     // card.  Units of one length (chosen pages, one sequence's rows) are shared while few and long: 8 units of 47 tiles 15 us and 14 whole,
     // of 125 15 and 27, 128 of 125 27 and 28, 256 of 188 53 and 48, 192 of 128 chosen 52 and 50.  Sequences of several lengths leave
     // a card of whole units uneven: 512 of up to 63 tiles 25 us and 20 whole, of up to 188 40 and 47, 2000 of up to 125 94 and 91, of up
     // to 313 188 and 209.
-    const bool shared = a.many ? busy < 2 * slots && tiles > 32
+    const bool shared = a.many ? busy < 1024 && tiles > 32
                         : top || bt.n_seqs == 1 ? units < 200 && tiles * (200 - units) > 9000
                                                 : tiles > 48 + units / 8;
     a.row_tiles = (uint32_t)row_tiles;
@@ -180,7 +182,7 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     uint64_t at = 0;
     if (top) {
         // Scores go by way of memory where LDS does not hold them, and where few tokens have many pages: all CUs score, 30 us for one
-        // sequence of 1024 pages against 33 by one workgroup a head, 53 against 55 for 32 sequences; 384 tokens of a prompt take 45 us
+        // sequence of 1024 pages against 33 by one workgroup a head, 53 against 55 for 32 sequences; 384 tokens of a prompt take 35 us
         // in LDS and 82 by way of memory.
         const bool split = bt.table_width > kChooseScores || (kv_max_pages(c, bt) > 512 && (uint64_t)bt.rows * c.heads <= 1024);
         // 256 pages a workgroup, 64 a wave; 128 where that leaves CUs idle (one sequence of 1024 pages, 8 heads: 31 and 29 us)
