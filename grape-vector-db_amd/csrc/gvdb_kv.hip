@@ -909,7 +909,8 @@ __device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j,
 // A workgroup takes 16 query rows of a unit and key head and one split of its tiles; its four waves take steps of them in
 // turn, one step's loads in flight while another is worked on, and join their parts through LDS.  With one query token a
 // sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it where there are many (32 sequences of 32 pages:
-// 18.5 us).  One sequence of 768 tokens takes 9 us, 4 of them before the first product (length, table, tiles, one behind the other).
+// 18.5 us).  One sequence of 768 tokens takes 9 us, of which its 24 tiles are 4; the rest is the chain of
+// loads before the first product (length, table, tiles), the join and the launch.
 // 384 tokens' own 40 pages of 32, 4 heads: 47 us, 5.7 TB/s out of the caches and three quarters of the cycles in vector instructions.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 : 3) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
@@ -961,7 +962,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
 // wave takes whole is written at once; the others' parts go to slot w + u (w and u only ever grow along the line: no two
 // parts share one) and are joined by k_kv_combine.  Waves never wait for one another, and loads run on over the borders
 // of units, the next unit's queries among them.  Bound by the reads: 4 sequences of 262144 tokens, 8 heads of 128 channels, 205 us with
-// the join, 5.6 TB/s; 64 of up to 10000, 57 us, 4.1 TB/s, of which 5 are the join and 5 the way to the first product.
+// the join, 5.6 TB/s; 64 of up to 10000, 57 us, 4.1 TB/s, of which the join is 5.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T);
