@@ -169,10 +169,10 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
         } else {
             // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 336 us,
-            // for 1024 of them 354, for 512 432), or 3072 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
+            // for 1024 of them 354, for 512 432), or 2560 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
             // 768 121).  Of 16 tiles at least, for 128 rows; of 16 rows a part's time grows with its tiles and the join's with the parts,
             // so of the square root of all tiles (best of 6 .. 32: 94 tiles 8 to 12, 250 12 to 16, 625 24, 938 32)
-            const uint64_t parts = a.many ? 2048 : 3072, least = a.many ? 16 : std::max<uint64_t>(8, (uint64_t)std::sqrt((double)tiles));
+            const uint64_t parts = a.many ? 2048 : 2560, least = a.many ? 16 : std::max<uint64_t>(8, (uint64_t)std::sqrt((double)tiles));
             a.chunk = (uint32_t)((std::max(least, (busy * tiles + parts - 1) / parts) + 1) / 2 * 2);  // whole steps
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         }
