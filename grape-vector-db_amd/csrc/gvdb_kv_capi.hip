@@ -150,7 +150,8 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     // of 125 15 and 27, 128 of 125 27 and 28, 256 of 188 53 and 48, 192 of 128 chosen 52 and 50.  Sequences of several lengths leave
     // a card of whole units uneven: 512 of up to 63 tiles 25 us and 20 whole, of up to 188 40 and 47, 2000 of up to 125 94 and 91, of up
     // to 313 188 and 209.
-    const bool shared = a.many ? busy < 1024 && tiles > 32
+    const bool known = !bt.cu || bt.n_seqs == 1;  // how many rows a sequence has
+    const bool shared = a.many ? known || (busy < 1024 && tiles > 32)
                         : top || bt.n_seqs == 1 ? units < 200 && tiles * (200 - units) > 9000
                                                 : tiles > 48 + units / 8;
     a.row_tiles = (uint32_t)row_tiles;
@@ -167,8 +168,21 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
             a.least = std::max<uint32_t>(4, (uint32_t)std::sqrt((double)tiles) / 4);
             a.slot_rows = (uint32_t)std::min<uint64_t>(16, rows_each);
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
+        } else if (a.many && known) {
+            // Workgroups of 128 rows that all have work run in rounds.  A round of m workgroups a CU takes about (m + 1) / 2 times what one
+            // of a single one does, 8 tiles' time before its first tile, and the join as much again: the number of parts that takes least
+            // (2 sequences of 300 tokens over 5000: 3 parts 116 us, 5 131, 1 180; 6 of 256 over 1500: 1 67, 3 93).
+            const uint64_t fit = slots / 256;
+            uint64_t best = ~0ull;
+            for (uint64_t k = 1; k <= std::max<uint64_t>(1, tiles / 16) && k <= 64; ++k) {
+                const uint64_t blocks = busy * k, rest = blocks % slots;
+                const uint64_t time = ((tiles + k - 1) / k + 8) * (blocks / slots * (fit + 1) + (rest ? (rest + 255) / 256 + 1 : 0)) + (k > 1 ? 16 : 0);
+                if (time < best) best = time, a.splits = (uint32_t)k;
+            }
+            a.chunk = (uint32_t)((tiles + a.splits - 1) / a.splits + 1) / 2 * 2;
+            a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         } else {
-            // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 336 us,
+            // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 333 us,
             // for 1024 of them 354, for 512 432), or 2560 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
             // 768 121).  Of 16 tiles at least, for 128 rows; of 16 rows a part's time grows with its tiles and the join's with the parts,
             // so of the square root of all tiles (best of 6 .. 32: 94 tiles 8 to 12, 250 12 to 16, 625 24, 938 32)
