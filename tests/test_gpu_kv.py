@@ -392,6 +392,19 @@ def test_attend_many_rows_in_parts(kv, dtype, Hq, heads, D, lens, new):
     check_attend(st, q, new, out, lse)
 
 
+@pytest.mark.parametrize("dtype,Hq,heads,D,lens,new", [("bf16", 32, 2, 64, (12500,), 32), ("f16", 16, 2, 128, (7000, 6500), 64),
+                                                       ("bf16", 16, 1, 256, (12400,), 64), ("f16", 24, 3, 64, (3300, 5000, 17, 0), 70)])
+def test_attend_many_rows_in_rounds(kv, dtype, Hq, heads, D, lens, new):
+    """As many rows each sequence: parts by rounds of workgroups.  Every 97th row and head is checked."""
+    st = Store(kv, 53, dtype, heads, D, 64, lens)
+    q = queries(54, dtype, (new,) * len(lens), Hq, D).cuda()
+    lse = torch.empty(q.shape[:2], device="cuda")
+    every = [(i, h) for i in range(len(q)) for h in range(Hq)]
+    for hints in ({"max_len": max(lens)}, {}, {"max_len": 500}):
+        out = st.cache.attend(q, st.table, st.lengths(), lse=lse, **hints)
+        check_attend(st, q, (new,) * len(lens), out, lse, skip=set(every) - set(every[::97]))
+
+
 @pytest.mark.parametrize("dtype,Hq,D,page", [("bf16", 2, 128, 64), ("f16", 2, 64, 32), ("bf16", 2, 256, 96), ("f16", 4, 128, 32)])
 def test_what_is_masked_in_a_crowd_may_hold_anything(kv, dtype, Hq, D, page):
     for poison in (float("nan"), float("inf"), -float("inf")):
