@@ -129,22 +129,33 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     const uint64_t units0 = top ? bt.rows : bt.n_seqs;
     // Workgroups that have rows, of `w` rows each: with `cu` the sequences are of several lengths, and `rows` says how many there are in all.
     auto busy_of = [&](uint64_t w, uint64_t n_units) { return std::min(n_units, (bt.rows * group / w + bt.n_seqs) * c.heads); };
-    // 128 rows and more share the values' expansion: a chunk of 2048 tokens takes 632 us so and 1110 us in tiles of 16 rows; at 64 rows
-    // a sequence 40 and 35 us, at 128 rows 49 and 50.  It wants three quarters of a workgroup a CU, parts of 512 tokens counted: 24 chunks
-    // of 64 tokens over 250 take 19 us so and 28 in tiles of 16 rows, 16 of them over 900 36 and 32, one of 512 over 2000 28 and 26, over
-    // 16000 33 and 37.  In 32 bits the pieces do not fit the registers: 130 and 117 us at 512 rows.
-    const uint64_t busy128 = busy_of(128, units0 * c.heads * ((rows_each + 127) / 128));
-    a.many = !top && dtype != GVDB_F32 && rows_each >= 128 && busy128 * (tiles > 32 ? tiles : 16) >= 16 * 192;
-    uint64_t row_tiles = a.many ? (rows_each + 127) / 128 : (rows_each + 15) / 16;
-    // grids stay below 2^20 tiles of rows where the hints are loose: the kernels stride over the rest
-    row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
-    const uint64_t units = units0 * c.heads * row_tiles;
-    const uint64_t busy = top ? units : busy_of(a.many ? 128 : 16, units);
     // As many workgroups as the card's registers hold at once: three a CU of 64 channels, two of 128, one of 256.  128 channels, 8 heads,
     // 64 sequences of up to 10000 tokens: 64 us with one, 58 with two, 66 with four; 4 x 262144 tokens: 230, 204, 237 us; 256 channels,
     // 4 heads, 64 sequences of up to 20000: 150 us with half a one, 96 with one, 102 with two; 64 channels, 8 heads: 66 us with two, 63
     // with three.
     const uint64_t slots = c.dim == 256 ? 256 : c.dim == 128 ? 512 : 768;
+    // Workgroups of 128 rows share the values' expansion, and run in rounds.  A round of m workgroups a CU takes about (m + 1) / 2 times
+    // what one of a single one does, 8 tiles' time before its first tile, and a join as much again; in units of half a tile, 0.42 us, with
+    // the number of parts that takes least (2 sequences of 300 tokens over 5000: 3 parts 116 us, 5 131, 1 180; 6 of 256 over 1500: 1 67,
+    // 3 93).
+    const uint64_t busy128 = busy_of(128, units0 * c.heads * ((rows_each + 127) / 128));
+    uint64_t time128 = ~0ull, parts128 = 1;
+    for (uint64_t k = 1; k <= std::max<uint64_t>(1, tiles / 16) && k <= 64; ++k) {
+        const uint64_t blocks = busy128 * k, rest = blocks % slots;
+        const uint64_t time = ((tiles + k - 1) / k + 8) * (blocks / slots * (slots / 256 + 1) + (rest ? (rest + 255) / 256 + 1 : 0)) + (k > 1 ? 16 : 0);
+        if (time < time128) time128 = time, parts128 = k;
+    }
+    // By 16 rows the card does 800 tiles (64 channels: 1000) in one of these units, 5 go by before a workgroup's first, and a join where
+    // they are too few to go whole.  16 sequences of 64 tokens over 900, 4 heads a group: 36 us by 128 rows, 27 by 16; 64 over 300 57 and
+    // 90; 2 over 16000 48 and 56; 2 of 2048 over 10000, 8 heads: 630 and 1110.  In 32 bits the pieces do not fit the registers: 130 and
+    // 117 us at 512 rows.
+    const uint64_t busy16 = busy_of(16, units0 * c.heads * ((rows_each + 15) / 16));
+    a.many = !top && dtype != GVDB_F32 && rows_each >= 128 && time128 < 5 + busy16 * (tiles + 5) / (c.dim == 64 ? 1000 : 800) + (busy16 < 512 ? 14 : 0);
+    uint64_t row_tiles = a.many ? (rows_each + 127) / 128 : (rows_each + 15) / 16;
+    // grids stay below 2^20 tiles of rows where the hints are loose: the kernels stride over the rest
+    row_tiles = std::max<uint64_t>(1, std::min<uint64_t>(row_tiles, (1ull << 20) / std::max<uint64_t>(1, units0 * c.heads) + 1));
+    const uint64_t units = units0 * c.heads * row_tiles;
+    const uint64_t busy = top ? units : busy_of(a.many ? 128 : 16, units);
     // Whole, a unit of 16 rows takes 6 us and 0.17 a tile; shared, all of them 14 us (the join's launch among it) and their share of the
     // card.  Units of one length (chosen pages, one sequence's rows) are shared while few and long: 8 units of 47 tiles 15 us and 14 whole,
     // of 125 15 and 27, 128 of 125 27 and 28, 256 of 188 53 and 48, 192 of 128 chosen 52 and 50.  Sequences of several lengths leave
@@ -169,16 +180,7 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
             a.slot_rows = (uint32_t)std::min<uint64_t>(16, rows_each);
             a.row_tiles = (uint32_t)((rows_each + 15) / 16);
         } else if (a.many && known) {
-            // Workgroups of 128 rows that all have work run in rounds.  A round of m workgroups a CU takes about (m + 1) / 2 times what one
-            // of a single one does, 8 tiles' time before its first tile, and the join as much again: the number of parts that takes least
-            // (2 sequences of 300 tokens over 5000: 3 parts 116 us, 5 131, 1 180; 6 of 256 over 1500: 1 67, 3 93).
-            const uint64_t fit = slots / 256;
-            uint64_t best = ~0ull;
-            for (uint64_t k = 1; k <= std::max<uint64_t>(1, tiles / 16) && k <= 64; ++k) {
-                const uint64_t blocks = busy * k, rest = blocks % slots;
-                const uint64_t time = ((tiles + k - 1) / k + 8) * (blocks / slots * (fit + 1) + (rest ? (rest + 255) / 256 + 1 : 0)) + (k > 1 ? 16 : 0);
-                if (time < best) best = time, a.splits = (uint32_t)k;
-            }
+            a.splits = (uint32_t)parts128;
             a.chunk = (uint32_t)((tiles + a.splits - 1) / a.splits + 1) / 2 * 2;
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         } else {
