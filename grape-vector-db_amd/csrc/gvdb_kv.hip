@@ -80,6 +80,10 @@ __device__ __forceinline__ void pack_pieces(float a, float b, uint32_t (&out)[NP
     }
 }
 
+// A pair of bf16 whose infinities become NaN: a query's infinity times keys of one sign would be scores of -inf, which read as masked.
+// (In more pieces the second is inf - inf.)
+__device__ __forceinline__ uint32_t inf_to_nan(uint32_t w) { return w | ((w & 0x7F807F80u) + 0x00800080u & 0x80008000u) >> 9; }
+
 // Largest value over the four lanes that hold one query row (n, n + 16, n + 32, n + 48).
 __device__ __forceinline__ float row_max(float v) {
     u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -787,7 +791,7 @@ struct RawQueries {
         for (int i = 0; i < D / 32 * 4; ++i) {
             uint32_t pc[NP];
             if constexpr (T == GVDB_BF16) {
-                pc[0] = r[i / 4][i % 4] ^ sign;
+                pc[0] = inf_to_nan(r[i / 4][i % 4] ^ sign);
             } else if constexpr (T == GVDB_F16) {
                 const uint32_t w = r[i / 4][i % 4] ^ sign;
                 pack_pieces<NP>((float)__builtin_bit_cast(_Float16, (uint16_t)w), (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)), pc);
@@ -1135,7 +1139,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_atte
                     uint32_t pc[NP];
                     pack_pieces<NP>(bits_f32(__float_as_uint(x[2 * e]) ^ sign), bits_f32(__float_as_uint(x[2 * e + 1]) ^ sign), pc);
 #pragma unroll
-                    for (int p = 0; p < NP; ++p) w.qf[p][ch][e] = pc[p];
+                    for (int p = 0; p < NP; ++p) w.qf[p][ch][e] = NP == 1 ? inf_to_nan(pc[p]) : pc[p];
                 }
             }
         }

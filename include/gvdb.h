@@ -605,12 +605,13 @@ gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batc
  * length - n + i + 1 of its length tokens, else all of them.  Query head h
  * reads key/value head h / (q_heads / kv_heads).  A row that sees no token is 0
  * (lse: -inf).  lse: device [rows][q_heads] f32, the natural logarithm of the
- * softmax's denominator, or NULL.  q and out: one type, q_heads heads; out's rows must not overlap, and out may
- * be q itself.  A row of q that is not finite spoils no other row.  Sums and
- * statistics are kept in 32 bits; keys, values and queries enter the products
- * exactly, the probabilities in 16 bits for bf16 and f16 rows (in 8 for prompts of
- * bf16 rows: from 128 rows a sequence on, a group's heads counted) and in 24
- * for f32. */
+ * softmax's denominator, or NULL.  q and out: one type, q_heads heads; out's
+ * rows must not overlap, and out may be q itself.  A row of q that holds an
+ * infinity or a NaN is NaN where it sees a token, and spoils no other row.
+ * Sums and statistics are kept in 32 bits; keys, values and queries enter the
+ * products exactly, the probabilities in 16 bits for bf16 and f16 rows (in 8
+ * for prompts of bf16 rows: from 128 rows a sequence on, a group's heads
+ * counted) and in 24 for f32. */
 gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
                                   uint32_t q_heads, float scale, int32_t causal, const gvdb_kv_rows* out, float* lse,
                                   void* scratch, uint64_t scratch_bytes, void* stream);
