@@ -39,6 +39,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kLowest = -3e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
 // Pieces of 8 bits that a type's values are split into for the products.
 constexpr int pieces(int dtype) { return dtype == GVDB_BF16 ? 1 : dtype == GVDB_F16 ? 2 : 3; }
+// Pieces of a probability, on every path alike: 16 bits for rows of 16 bits, 24 for those of 32.  With one piece for
+// bf16 rows half of an output's error would be the probabilities', and the size of a launch would decide how many bits a row gets.
+template <int NP>
+constexpr int kProbPieces = NP < 2 ? 2 : NP;
 // The value, as one that the compiler knows nothing of: what is reckoned from it in a branch that is seldom taken stays in
 // that branch, and takes no registers outside.
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
@@ -691,7 +695,7 @@ struct Step {  // a tile whose loads were issued
 // sequences of 1500 tokens take 26 us so, 22 tile by tile; 4 of 262144 215 and 205.
 template <int D, int NP, bool CHOSEN>
 __device__ __forceinline__ void work_step(Rows<D, NP>& w, Step<D>& st, const Job<CHOSEN>& j, float c2, uint32_t lane) {
-    constexpr int PP = NP < 2 ? 2 : NP;  // of a probability: with one, half of a bf16 row's error would be the probabilities'
+    constexpr int PP = kProbPieces<NP>;
     f4 s[2];
     tile_scores<D, NP>(w, st.t, s);
     const bool plain = st.there && (int64_t)st.base + 32 <= j.least;
@@ -1059,8 +1063,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_kv_att
 // A row of keys stands for token t(row) with bits 2 and 3 exchanged, so that S^T leaves a lane with eight neighbouring
 // tokens of its query row, which O^T = V^T P^T takes as they are.  Channel j of sixteenth l lies at row 16 j + l of V^T.
 // Bound by the vector instructions that expand keys and reckon probabilities: 2048 tokens of 2 sequences over 10000, 32 heads on 8 of
-// 128 channels, 630 us, 950 TFLOP/s; vector instructions issue in 64 % of the cycles, the matrix units are busy in 41 %, and two
-// workgroups a CU, all that the registers hold, overlap them no further.
+// 128 channels, 839 us, 720 TFLOP/s (with probabilities of 8 bits, whose products are half as many, 639 us); two workgroups a CU, all
+// that the registers hold, overlap them and the products no further.
 template <int D, int NP>
 struct Rows32 {
     u4 qf[NP][D / 16];  // query pieces: lane 32 i + n has row n, channels [i D/2, (i+1) D/2)
@@ -1095,11 +1099,10 @@ __device__ __forceinline__ void load_keys32(const uint8_t* p, uint32_t i, uint32
 }
 
 // Rows of 16 bits only: in 32 bits the pieces of 32 rows do not fit the registers.
-// Probabilities of bf16 rows are in one piece here, where a second one's products would cost a third of the time; the bound on
-// workgroups keeps D = 64 within a third of the registers (55 -> 52 us: 2 sequences of up to 500 tokens, f16).
+// The bound on workgroups keeps D = 64 within a third of the registers (55 -> 52 us: 2 sequences of up to 500 tokens, f16).
 template <int D, int T>
 __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_attend_rows(KvCache c, KvBatch bt, AttendArgs a) {
-    constexpr int NP = pieces(T), W = D / 16, G = D / 32;
+    constexpr int NP = pieces(T), PP = kProbPieces<NP>, W = D / 16;
     __shared__ u4 s_v[2][8 * D];
     __shared__ uint32_t s_odd[2][4];
     clear_rest<D, T>(c, bt, a);
@@ -1294,7 +1297,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_atte
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int ch = 0; ch < 2; ++ch) {
-                    u4 v[D / 32], pf[NP];  // the values are read while the probabilities are reckoned
+                    u4 v[D / 32], pf[PP];  // the values are read while the probabilities are reckoned
 #pragma unroll
                     for (int k = 0; k < D / 32; ++k) v[k] = s_v[buf][(4 * x + 2 * ch + i2) * D + 32 * k + n32];
                     __builtin_amdgcn_sched_barrier(0);
@@ -1302,16 +1305,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_atte
                     for (int e = 0; e < 4; ++e) {
                         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * ch + 2 * e], a.scale_log2, -top));
                         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * ch + 2 * e + 1], a.scale_log2, -top));
-                        uint32_t pc[NP];
-                        pack_pieces<NP>(p0, p1, pc);
+                        uint32_t pc[PP];
+                        pack_pieces<PP>(p0, p1, pc);
                         w.l += p0 + p1;  // of the probabilities as they are: the row's logarithm is given out
 #pragma unroll
-                        for (int p = 0; p < NP; ++p) pf[p][e] = pc[p];
+                        for (int p = 0; p < PP; ++p) pf[p][e] = pc[p];
                     }
 #pragma unroll
                     for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-                        for (int p = 0; p < NP; ++p)
+                        for (int p = 0; p < PP; ++p)
                             w.o[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v[k]), as_bf8(pf[p]), w.o[k], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }

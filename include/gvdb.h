@@ -609,9 +609,8 @@ gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batc
  * rows must not overlap, and out may be q itself.  A row of q that holds an
  * infinity or a NaN is NaN where it sees a token, and spoils no other row.
  * Sums and statistics are kept in 32 bits; keys, values and queries enter the
- * products exactly, the probabilities in 16 bits for bf16 and f16 rows (in 8
- * for prompts of bf16 rows: from 128 rows a sequence on, a group's heads
- * counted) and in 24 for f32. */
+ * products exactly, the probabilities in 16 bits for bf16 and f16 rows and in
+ * 24 for f32, whatever the hints and the other sequences of the batch are. */
 gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
                                   uint32_t q_heads, float scale, int32_t causal, const gvdb_kv_rows* out, float* lse,
                                   void* scratch, uint64_t scratch_bytes, void* stream);
