@@ -99,11 +99,26 @@ gvdb_status take_rows(const gvdb_kv_rows* in, const char* what, KvRows& r) {
     return GVDB_OK;
 }
 
+// Whether two of [rows][heads] runs of d elements share an element: their starts lie i * rs + j * hs apart, |i| < rows, |j| < heads.
+bool overlapping(uint64_t rows, uint64_t heads, int64_t row_stride, int64_t head_stride, uint64_t d) {
+    typedef unsigned __int128 wide;
+    auto size = [](int64_t x) { return x < 0 ? 0 - (uint64_t)x : (uint64_t)x; };
+    const uint64_t rs = size(row_stride), hs = size(head_stride);
+    if ((rows > 1 && rs < d) || (heads > 1 && hs < d)) return true;
+    if (rows < 2 || heads < 2 || rs >= (wide)(heads - 1) * hs + d || hs >= (wide)(rows - 1) * rs + d) return false;
+    // one inside the other, otherwise than [rows][heads] or [heads][rows]: both strides are d or more, so only i and j whose offsets
+    // take from one another can meet, and for each head the two rows next to it
+    for (uint64_t j = 1; j < heads; ++j) {
+        const wide at = (wide)j * hs, i = at / rs;
+        if ((i < rows && at - i * rs < d) || (i + 1 < rows && (i + 1) * rs - at < d)) return true;
+    }
+    return false;
+}
+
 // Rows that are written lie apart: two that share an element would be written in any order.
 gvdb_status take_out(const gvdb_kv_rows* in, const char* what, const KvCache& c, uint32_t rows, uint32_t heads, KvRows& r) {
     if (gvdb_status s = take_rows(in, what, r)) return s;
-    const int64_t d = c.dim;
-    if ((rows > 1 && r.row_stride > -d && r.row_stride < d) || (heads > 1 && r.head_stride > -d && r.head_stride < d))
+    if (overlapping(rows, heads, r.row_stride, r.head_stride, c.dim))
         return invalid((std::string("token cache: overlapping rows of ") + what).c_str());
     return GVDB_OK;
 }
@@ -245,8 +260,8 @@ gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const
     Plan p;
     KvRows qr, orow;
     if (gvdb_status s = take_rows(q, "q", qr)) return s;
-    if (gvdb_status s = take_out(out, "out", call.c, call.bt.rows, q_heads, orow)) return s;
     if (gvdb_status s = plan_attend(call.c, call.bt, qr.dtype, q_heads, choose ? top : 0, p)) return s;
+    if (gvdb_status s = take_out(out, "out", call.c, call.bt.rows, q_heads, orow)) return s;
     p.a.q = qr, p.a.out = orow;
     if (p.a.q.dtype != p.a.out.dtype) return invalid("token cache: q and out are of one dtype");
     if (p.bytes && !scratch) return invalid("token cache: null scratch");

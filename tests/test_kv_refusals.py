@@ -1,0 +1,44 @@
+"""CPU: calls of the token cache that are refused, and those beside them that are not (no HIP call is made)."""
+import ctypes as C
+import itertools
+
+import pytest
+
+from test_kv import ARG, call  # noqa: F401  (call: the fixture)
+
+
+def overlap(rows, heads, rs, hs, d):
+    starts = [i * rs + j * hs for i, j in itertools.product(range(rows), range(heads))]
+    return any(abs(a - b) < d for a, b in itertools.combinations(starts, 2))
+
+
+@pytest.mark.parametrize("rows,heads", [(4, 4), (3, 2), (2, 6), (1, 4), (4, 2)])
+def test_outputs_overlap_in_no_two_rows(call, rows, heads):  # noqa: F811
+    """Both strides together decide it: a row's next head may be the next row's first."""
+    call.batch.n_seqs, call.batch.rows = 1, rows
+    call.batch.table_width = call.batch.table_stride = 5000
+    rc, need = call.size(heads=heads)
+    assert rc == 0 and need > 0
+    seen = set()
+    for rs, hs in itertools.product((128, -128, 129, 200, 255, 256, 300, -384, 512, 640, 1000, 4096), repeat=2):
+        call.out.row_stride, call.out.head_stride = rs, hs
+        # one that is in order gets as far as the scratch, which is a byte too small
+        assert call.attend(heads=heads, size=need - 1) == ARG
+        bad = overlap(rows, heads, rs, hs, 128)
+        assert ("overlapping" if bad else "scratch") in call.why(), (rs, hs)
+        seen.add(bad)
+        if rows > 1 and heads == 2:
+            call.rows.row_stride, call.rows.head_stride = rs, hs
+            if bad:
+                rc = call.L.gvdb_kv_read_device(C.byref(call.cache), C.byref(call.batch), C.byref(call.rows), None, None)
+                assert rc == ARG and "overlapping" in call.why()
+    assert seen == ({False} if rows == 1 else {False, True})
+
+
+def test_strides_of_any_size(call):  # noqa: F811
+    call.batch.table_width = call.batch.table_stride = 5000
+    need = call.size()[1]
+    for rs, hs, bad in ((-(1 << 63), 1 << 62, True), (1 << 62, -(1 << 63), True), (1 << 62, 1 << 62, True), (-(1 << 63), -(1 << 63), True),
+                        ((1 << 63) - 1, -(1 << 63), True), (3 << 60, 1 << 62, False), (-(1 << 63), 1000, False), (128, -(1 << 63), False)):
+        call.out.row_stride, call.out.head_stride = rs, hs
+        assert call.attend(size=need - 1) == ARG and ("overlapping" if bad else "scratch") in call.why(), (rs, hs)
