@@ -597,7 +597,10 @@ gvdb_status gvdb_kv_append_device(const gvdb_kv_cache* cache, const gvdb_kv_batc
  * k or v may be NULL.  Output rows and heads must not overlap. */
 gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* k,
                                 const gvdb_kv_rows* v, void* stream);
-/* Scratch of the attention calls (top: 0 for gvdb_kv_attend_device). */
+/* Scratch of an attention call (top: 0 for gvdb_kv_attend_device): a rule on the
+ * cache, the batch's sizes and its hints, reckoned on the host without the
+ * device.  It is asked for each call: a smaller batch may take more, where few
+ * rows share what many would each have to themselves. */
 gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t q_heads,
                                   uint32_t top, uint64_t* bytes);
 /* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the tokens that

@@ -42,3 +42,37 @@ def test_strides_of_any_size(call):  # noqa: F811
                         ((1 << 63) - 1, -(1 << 63), True), (3 << 60, 1 << 62, False), (-(1 << 63), 1000, False), (128, -(1 << 63), False)):
         call.out.row_stride, call.out.head_stride = rs, hs
         assert call.attend(size=need - 1) == ARG and ("overlapping" if bad else "scratch") in call.why(), (rs, hs)
+
+
+@pytest.mark.parametrize("top,new,width", [(0, 1, 64), (0, 5, 64), (0, 200, 300), (16, 1, 64), (16, 3, 2000)])
+def test_scratch_is_asked_for_each_call(call, top, new, width):  # noqa: F811
+    """The answer is what the same call takes, for every batch and length on the way down; a smaller batch may need more."""
+    call.cache.kv_heads, call.batch.table_width, call.batch.table_stride = 8, width, width
+    call.q.row_stride = call.out.row_stride = 32 * 128
+    sizes = {}
+    for seqs, max_len, cu in itertools.product((64, 33, 16, 8, 5, 2, 1), (width * 64, 1536, 300, 1), (None, 4096)):
+        call.batch.n_seqs, call.batch.rows, call.batch.max_new = seqs, seqs * new, new
+        call.batch.max_len, call.batch.cu = max_len, cu
+        rc, need = call.size(heads=32, top=top)
+        assert rc == 0
+        sizes[seqs, max_len, cu] = need
+
+        def why(size):  # at an address that every call refuses, once the size is enough
+            out = []
+            for dtype in (0, 1, 2):
+                call.q.dtype = call.out.dtype = dtype
+                args = (C.byref(call.cache), C.byref(call.batch), C.byref(call.q), 32, 0.1)
+                end = (4100, size, None)
+                if top:
+                    rc = call.L.gvdb_kv_attend_topk_device(*args, top, 1, 1, C.byref(call.out), None, None, *end)
+                else:
+                    rc = call.L.gvdb_kv_attend_device(*args, 1, C.byref(call.out), None, *end)
+                assert rc == ARG
+                out.append("aligned" if "aligned" in call.why() else "below" if "below" in call.why() else call.why())
+            return out
+
+        assert why(need) == ["aligned"] * 3
+        if need:
+            assert "below" in why(need - 1)
+    if new == 1 and not top:
+        assert sizes[64, 1536, None] == 0 < sizes[1, 1536, None]
