@@ -348,6 +348,25 @@ gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batc
     });
 }
 
+gvdb_status gvdb_kv_attend_path(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t dtype, uint32_t q_heads,
+                                uint32_t top, uint32_t* path) {
+    return guarded([&]() -> gvdb_status {
+        if (!path) return invalid("token cache: null path");
+        *path = GVDB_KV_UNITS;
+        KvCache c{};
+        KvBatch bt{};
+        if (gvdb_status s = take_cache(cache, c)) return s;
+        if (gvdb_status s = take_batch(batch, c, bt)) return s;
+        if (dtype > GVDB_BF16) return invalid("token cache: unknown dtype");
+        if (bt.rows == 0) return GVDB_OK;
+        Plan p;
+        if (gvdb_status s = plan_attend(c, bt, dtype, q_heads, top, p)) return s;
+        const bool parts = p.a.splits > 1;
+        *path = p.a.lanes ? GVDB_KV_LINE : p.a.many ? (parts ? GVDB_KV_ROW_PARTS : GVDB_KV_ROWS) : parts ? GVDB_KV_PARTS : GVDB_KV_UNITS;
+        return GVDB_OK;
+    });
+}
+
 gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q, uint32_t q_heads,
                                   float scale, int32_t causal, const gvdb_kv_rows* out, float* lse, void* scratch,
                                   uint64_t scratch_bytes, void* stream) {

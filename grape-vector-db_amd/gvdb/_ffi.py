@@ -214,6 +214,7 @@ SIGNATURES = {
     "gvdb_kv_append_device": (C.c_int, [P, P, P, P, P]),
     "gvdb_kv_read_device": (C.c_int, [P, P, P, P, P]),
     "gvdb_kv_scratch_bytes": (C.c_int, [P, P, u32, u32, PU64]),
+    "gvdb_kv_attend_path": (C.c_int, [P, P, u32, u32, u32, PU32]),
     "gvdb_kv_attend_device": (C.c_int, [P, P, P, u32, f32, i32, P, P, P, u64, P]),
     "gvdb_kv_attend_topk_device": (C.c_int, [P, P, P, u32, f32, u32, u32, u32, P, P, P, P, u64, P]),
 }

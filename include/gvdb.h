@@ -603,6 +603,18 @@ gvdb_status gvdb_kv_read_device(const gvdb_kv_cache* cache, const gvdb_kv_batch*
  * rows share what many would each have to themselves. */
 gvdb_status gvdb_kv_scratch_bytes(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t q_heads,
                                   uint32_t top, uint64_t* bytes);
+/* Which way an attention call of these sizes and hints would go (dtype: of its
+ * rows), for tests and for tuning hints: all give the same results but for the
+ * order of 32-bit sums. */
+typedef enum gvdb_kv_path {
+    GVDB_KV_UNITS = 0,     /* 16 rows a workgroup, over everything that they see */
+    GVDB_KV_PARTS = 1,     /* the same over parts of it, joined */
+    GVDB_KV_LINE = 2,      /* 16 rows a wave, equal shares of all tiles, joined */
+    GVDB_KV_ROWS = 3,      /* 128 rows a workgroup */
+    GVDB_KV_ROW_PARTS = 4  /* the same over parts, joined */
+} gvdb_kv_path;
+gvdb_status gvdb_kv_attend_path(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, uint32_t dtype, uint32_t q_heads,
+                                uint32_t top, uint32_t* path);
 /* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the tokens that
  * row r sees: with `causal`, row i of a sequence's n sees the first
  * length - n + i + 1 of its length tokens, else all of them.  Query head h

@@ -1,12 +1,30 @@
 """GPU: what every path of the token cache's attention has to keep alike, whatever the launch was sized for."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import kv_plain as plain
-from test_gpu_kv import DT, HALF, TINY, i32, kv  # noqa: F401  (kv: the fixture)
+import test_gpu_kv
+from test_gpu_kv import DT, HALF, TINY, Store, check_attend, i32, kv, queries  # noqa: F401  (kv: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+UNITS, PARTS, LINE, ROWS, ROW_PARTS = range(5)  # enum gvdb_kv_path
+
+
+@pytest.fixture(autouse=True)
+def sixteen_bits(monkeypatch):
+    """What `check_attend` allows for the probabilities' bits: bf16 rows have as many as f16's on every path."""
+    monkeypatch.setitem(test_gpu_kv.PROB, "bf16", 2.0 ** -16)
+
+
+def path(cache, q, table, lens, cu=None, max_new=0, max_len=0, top=0):
+    batch, _ = cache._batch(table, lens, cu, q.shape[0], max_new, max_len)
+    got = ctypes.c_uint32(99)
+    assert cache._lib.gvdb_kv_attend_path(cache._ref, batch, cache._codes[q.dtype], q.shape[1], top, ctypes.byref(got)) == 0
+    return got.value
 
 
 class Cancelling:
@@ -75,3 +93,133 @@ def test_probabilities_have_16_bits_on_every_path(kv, dtype, D, heads, group, pa
                 st.check(st.cache.attend(q, table, lens, cu=cu, causal=False, **hints), group)
         if rows == 1:  # every page chosen
             st.check(st.cache.attend_topk(q, table, lens, -(-n // page))[0], group)
+
+
+# ---- 128 rows a workgroup ---------------------------------------------------------------------
+class Crowd:
+    """The sequences of a Store `copies` times over, between `before` and `behind` rows of no sequence: enough rows for workgroups of
+    128, or (ROW_PARTS) a table far wider than the sequences.  Every copy's outputs are the first's bits, and the first is checked."""
+
+    def __init__(self, kv, want, seed, dtype, Hq, heads, D, page, lens, new, copies, before=0, behind=0):  # noqa: F811
+        width = 4000 if want == ROW_PARTS else None
+        self.st = Store(kv, seed, dtype, heads, D, page, lens, width=width)
+        self.cache, self.dtype, self.new, self.copies, self.want = self.st.cache, dtype, tuple(new), copies, want
+        one = queries(seed + 1, dtype, new, Hq, D)
+        rest = queries(seed + 2, dtype, (before + behind + 1,), Hq, D)
+        self.one, self.rows, self.before, self.behind = one.cuda(), len(one), before, behind
+        self.q = torch.cat((rest[:before], one.repeat(copies, 1, 1), rest[before:before + behind])).cuda()
+        self.table, self.lens = self.st.table.repeat(copies, 1), self.st.lengths().repeat(copies)
+        self.cu = i32((before + np.cumsum((0,) + self.new * copies)).tolist())
+        self.hints = {"max_new": max(new)} if want == ROW_PARTS else {"max_new": max(new), "max_len": max(max(lens), 1)}
+
+    def attend(self, q=None, lens=None, table=None, want=None, **more):
+        q, lens, table = self.q if q is None else q, self.lens if lens is None else lens, self.table if table is None else table
+        more = {**self.hints, **more}
+        assert path(self.cache, q, table, lens, self.cu, more["max_new"], more.get("max_len", 0)) == (self.want if want is None else want)
+        return self.cache.attend(q, table, lens, cu=self.cu, **more)
+
+    def first(self, x):
+        """The first copy's rows of x, after a look at the others."""
+        x = x[self.before:self.before + self.copies * self.rows].contiguous()
+        bits = x.view(torch.int16 if x.element_size() == 2 else torch.int32).view(self.copies, self.rows, *x.shape[1:])
+        assert torch.equal(bits, bits[:1].expand_as(bits))
+        return x[:self.rows]
+
+    def check(self, out, lse=None, skip=(), **more):
+        check_attend(self.st, self.one, self.new, self.first(out), None if lse is None else self.first(lse), skip=skip, **more)
+
+
+CROWDS = [  # (path, dtype, query heads, heads, channels, page, lengths, rows, copies): rows before their sequence's first token among them
+    (ROWS, "bf16", 16, 1, 64, 32, (150, 30, 0), (64, 40, 64), 32),
+    (ROWS, "f16", 8, 2, 128, 64, (400, 9), (128, 70), 32),
+    (ROWS, "bf16", 32, 1, 128, 96, (200, 64), (40, 31), 48),
+    (ROWS, "f16", 32, 1, 256, 64, (130, 20), (64, 61), 16),
+    (ROW_PARTS, "bf16", 32, 1, 64, 64, (600, 20), (40, 33), 1),
+    (ROW_PARTS, "f16", 32, 2, 128, 64, (3000, 100), (16, 9), 1),
+    (ROW_PARTS, "bf16", 32, 1, 256, 64, (1100, 5), (20, 9), 1),
+]
+
+
+@pytest.mark.parametrize("shape", CROWDS)
+def test_rows_strided_misaligned_and_outside(kv, shape):  # noqa: F811
+    """Queries inside a fused row and off 16 bytes, outputs inside wider rows, rows of no sequence at both ends: what is beside stays."""
+    c = Crowd(kv, shape[0], 70, *shape[1:], before=3, behind=5)
+    rows, Hq, D = c.q.shape
+    fused = torch.zeros(rows, Hq + 3, D, dtype=c.q.dtype, device="cuda")
+    fused[:, 1:Hq + 1] = c.q
+    flat = torch.zeros(rows * Hq * D + 1, dtype=c.q.dtype, device="cuda")[1:].view(rows, Hq, D)
+    flat.copy_(c.q)
+    heads_first = c.q.transpose(0, 1).contiguous().transpose(0, 1)
+    outside = [*range(3), *range(rows - 5, rows)]
+    for q in (fused[:, 1:Hq + 1], flat, heads_first):
+        big = torch.full((rows, Hq, D + 5), 3.0, dtype=q.dtype, device="cuda")
+        lse = torch.full((rows, Hq), 3.0, device="cuda")
+        c.check(c.attend(q, out=big[:, :, 2:D + 2], lse=lse), lse)
+        assert (big[outside] == 3).all() and (big[:, :, :2] == 3).all() and (big[:, :, D + 2:] == 3).all() and (lse[outside] == 3).all()
+        lse.fill_(3.0)
+        out = c.attend(q, lse=lse)  # the call's own output: rows of no sequence are 0, their logarithm -inf
+        c.check(out, lse)
+        assert (out[outside] == 0).all() and (lse[outside] == -np.inf).all()
+
+
+@pytest.mark.parametrize("shape", CROWDS)
+def test_rows_with_any_scale_and_mask(kv, shape):  # noqa: F811
+    c = Crowd(kv, shape[0], 73, *shape[1:])
+    for scale, causal in ((-0.2, True), (-0.05, False), (0.0, True), (0.4, False)):
+        lse = torch.empty(c.q.shape[:2], device="cuda")
+        c.check(c.attend(scale=scale, causal=causal, lse=lse), lse, scale=scale, causal=causal)
+
+
+@pytest.mark.parametrize("shape", CROWDS)
+def test_rows_write_over_their_queries(kv, shape):  # noqa: F811
+    c = Crowd(kv, shape[0], 76, *shape[1:])
+    want, own = c.attend(), c.q.clone()
+    assert c.attend(own, out=own) is own and torch.equal(own, want)
+
+
+@pytest.mark.parametrize("shape", CROWDS)
+def test_rows_by_any_hint(kv, shape):  # noqa: F811
+    """Lengths and rows beyond the hints that the launch was sized for, as a replayed graph has them."""
+    c = Crowd(kv, shape[0], 79, *shape[1:])
+    seen = set()
+    for hints in ({}, {"max_new": 1, "max_len": 1}, {"max_new": 20, "max_len": 64}, {"max_new": 4000000000, "max_len": 4000000000},
+                  {"max_new": max(c.new), "max_len": 1}, c.hints):
+        lse = torch.empty(c.q.shape[:2], device="cuda")
+        c.check(c.cache.attend(c.q, c.table, c.lens, cu=c.cu, lse=lse, **hints), lse)
+        seen.add(path(c.cache, c.q, c.table, c.lens, c.cu, **hints))
+    assert c.want in seen and len(seen) > 1
+
+
+@pytest.mark.parametrize("shape", [
+    (ROWS, "bf16", 16, 1, 64, 32, (150, 70), (64, 60), 48), (ROWS, "f16", 8, 2, 128, 64, (390, 70), (128, 70), 32),
+    (ROWS, "bf16", 32, 1, 256, 64, (130, 40), (64, 60), 16), (ROW_PARTS, "bf16", 32, 1, 64, 128, (150, 40), (64, 33), 1),
+    (ROW_PARTS, "f16", 32, 2, 128, 128, (150, 40), (64, 33), 1), (ROW_PARTS, "bf16", 32, 1, 256, 128, (150, 40), (64, 33), 1)])
+def test_rows_of_pages_that_are_not_there(kv, shape):  # noqa: F811
+    """A page that is not there, and a length that the table does not cover: NaN in the rows that see it, and in no other."""
+    c = Crowd(kv, shape[0], 82, *shape[1:])
+    S, L, n, page, width = len(c.st.lens), c.st.lens[0], c.new[0], c.st.page, c.table.shape[1]
+    for kind in (-1, c.cache.n_pages, "short table"):
+        table, lens = c.table.clone(), c.lens.clone()
+        if kind == "short table":  # every copy's first sequence ends two tokens behind its table, whose pages are all there
+            lens[::S] = width * page + 2
+            table[::S, L // page:] = table[0, 0]  # whole, and written
+            gone = torch.arange(n) >= n - 2
+        else:
+            table[::S, 1] = kind
+            gone = torch.arange(n) + L - n >= page
+        out = c.first(c.attend(lens=lens, table=table))
+        assert torch.isnan(out[:n]).flatten(1).all(1).tolist() == gone.tolist(), kind
+        assert torch.isfinite(out[:n][~gone]).all()
+        check_attend(c.st, c.one, c.new, out, skip={(r, h) for r in range(n) for h in range(c.q.shape[1]) if gone[r] or kind == "short table"})
+
+
+def test_paths_of_the_other_tests(kv):  # noqa: F811
+    """The ways that short calls take: single tokens, few tokens, packed rows, one sequence's prompt in 32 bits."""
+    cache = kv.KvCache(8, 8, 128, 64)
+    for dtype, seqs, new, width, ragged, max_len, want in (("bf16", 1, 1, 12, False, 768, UNITS), ("bf16", 64, 1, 157, False, 10000, LINE),
+                                                            ("f32", 5, 5, 300, True, 19000, PARTS), ("bf16", 2, 2048, 157, False, 10000, ROWS),
+                                                            ("f16", 2, 512, 500, True, 32000, ROW_PARTS), ("f32", 2, 2048, 157, False, 10000, UNITS)):
+        q = torch.empty(seqs * new, 32, 128, dtype=DT[dtype], device="cuda")
+        table, lens = torch.zeros(seqs, width, dtype=torch.int32, device="cuda"), i32([0] * seqs)
+        cu = i32((np.arange(seqs + 1) * new).tolist()) if ragged else None
+        assert path(cache, q, table, lens, cu, new, max_len) == want, (dtype, seqs, new)
