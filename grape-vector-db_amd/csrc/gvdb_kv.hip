@@ -891,7 +891,7 @@ __device__ __forceinline__ void join_waves(JoinLds<D>& s, Rows<D, NP>& w, const 
             for (int i = 0; i < 4; ++i) x[i] += u[i] * f, x[4 + i] += v[i] * f;
         }
         const int row = j.first + (int)r;
-        write_row<D, T>(a, j, row, d, x, m, l, a.splits > 1,
+        write_row<D, T>(a, j, row, d, x, m, l, !CHOSEN && a.splits > 1,
                         ((uint64_t)j.token_of(row) * a.q_heads + j.head_of(row)) * a.splits + split);
     }
     __syncthreads();
@@ -926,14 +926,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
     __shared__ JoinLds<D> s;
     clear_rest<D, T>(c, bt, a);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % a.splits;
-    const uint32_t rest = blockIdx.x / c.heads / a.splits;
+    const uint32_t splits = CHOSEN ? 1 : a.splits;  // chosen pages go whole here
+    const uint32_t h = blockIdx.x % c.heads, split = blockIdx.x / c.heads % splits;
+    const uint32_t rest = blockIdx.x / c.heads / splits;
     for (uint32_t row_tile = rest % a.row_tiles;; row_tile += a.row_tiles) {
         Job<CHOSEN> j;
         if (!j.set(c, bt, a, rest / a.row_tiles, row_tile, h, lane & 15u) || j.first >= j.rows) return;
         const uint32_t tiles = j.tiles(c, bt, a), s0 = (uint32_t)min((uint64_t)split * a.chunk, (uint64_t)tiles);
-        const uint32_t s1 = split + 1 == a.splits ? tiles : min(s0 + a.chunk, tiles);
-        if (a.splits > 1 && s0 >= s1) continue;  // no part: k_kv_combine does not read it
+        const uint32_t s1 = split + 1 == splits ? tiles : min(s0 + a.chunk, tiles);
+        if (splits > 1 && s0 >= s1) continue;  // no part: k_kv_combine does not read it
         Rows<D, NP> w;
         clear(w);
         RawQueries<D, T> raw;
@@ -1380,6 +1381,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void k_kv_atte
 // every so many-th part; the order of the sum is the lanes', alike on every run.  Bound by its chain of loads: 4 to 7 us.
 template <int D, int T, bool CHOSEN, bool FEW>
 __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, AttendArgs a) {
+    static_assert(!CHOSEN || !FEW, "chosen pages are joined along the line only");
     constexpr uint32_t L = D / 8, G = 64 / L;
     const uint32_t lane = threadIdx.x & 63u, g = lane / L, d = lane % L * 8;
     const uint64_t wave = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6), at = FEW ? wave * G + g : wave;
@@ -1392,7 +1394,7 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
     seq_rows(bt, b, r0, n);
     uint64_t first, step;  // where the parts lie
     uint32_t parts;
-    if (!FEW && a.lanes > 0) {
+    if (CHOSEN || (!FEW && a.lanes > 0)) {  // the line's
         const uint32_t group = a.q_heads / c.heads;
         const uint32_t row = (CHOSEN ? 0u : (uint32_t)(token - r0)) * group + head % group;
         const uint32_t u = (CHOSEN ? (uint32_t)token : b) * a.row_tiles + row / 16;
@@ -1406,7 +1408,7 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
     } else {
         const int64_t len = max(bt.lengths[b], 0);
         const int64_t limit = a.causal ? len - n + (token - r0) + 1 : len;
-        const uint32_t tiles = CHOSEN ? (uint32_t)min((int64_t)a.top, a.pages_seen(c, bt, limit)) * (c.page >> 5) : tiles_of(c, bt, limit);
+        const uint32_t tiles = tiles_of(c, bt, limit);
         parts = min(a.splits, (tiles + a.chunk - 1) / a.chunk);
         step = 1;
         first = at * a.splits;
@@ -1946,10 +1948,8 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
     const uint32_t chunks = fused ? 1 : (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
     const uint64_t others = (uint64_t)c.heads * chunks * bt.n_seqs;
     const uint32_t tok_tiles = capped(((uint64_t)bt.max_new + per - 1) / per, others, 1u << 22);
-    const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : a.splits * a.row_tiles * bt.rows);
-    const bool few = !a.lanes && a.splits <= 16;
-    const uint64_t per_join = few ? 4 * (512 / c.dim) : 4, joins = ((uint64_t)bt.rows * a.q_heads + per_join - 1) / per_join;
-    if (!fits(others * tok_tiles, kChooseThreads) || !fits(blocks) || !fits(joins) || (!fused && !fits((uint64_t)bt.rows * c.heads, kChooseThreads)))
+    const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : (uint64_t)a.row_tiles * bt.rows);
+    if (!fits(others * tok_tiles, kChooseThreads) || !fits(blocks) || (!fused && !fits((uint64_t)bt.rows * c.heads, kChooseThreads)))
         return hipErrorInvalidValue;
     if (fused) {
         const uint32_t lds = per * bt.table_width * 4;
@@ -1976,12 +1976,9 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));
     }
     GVDB_LAUNCH_CHECK();
-    if (a.lanes || a.splits > 1) {
-        if (few) {
-            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true, true><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
-        } else {
-            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true, false><<<(uint32_t)joins, 256, 0, s>>>(c, bt, a)));
-        }
+    if (a.lanes) {  // few units: a row and head a wave
+        const uint32_t joins = (bt.rows * a.q_heads + 3) / 4;
+        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_combine<D, T, true, false><<<joins, 256, 0, s>>>(c, bt, a)));
         GVDB_LAUNCH_CHECK();
     }
     return hipSuccess;

@@ -186,6 +186,7 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     if (shared) {
         const uint64_t line = units0 * ((rows_each + 15) / 16);
         const uint64_t most = line * (top ? (uint64_t)top : (uint64_t)bt.table_width + 1) * (c.page / 32);
+        // chosen pages: fewer than 200 units of at most 65536 pages of 32 tiles, so that a call that shares takes the line
         if (!a.many && (top || !bt.cu) && line <= kMaxUnits && most < (1ull << 31)) {
             // the rows of a unit are known: every wave gets the same share of all tiles, of 4 at least; of long sequences more, for the
             // join's sake, as below (8 heads, one sequence of 125 tiles: 13 us by 4, 16 by 8; of 938 26 and 21)

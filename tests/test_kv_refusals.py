@@ -76,3 +76,20 @@ def test_scratch_is_asked_for_each_call(call, top, new, width):  # noqa: F811
             assert "below" in why(need - 1)
     if new == 1 and not top:
         assert sizes[64, 1536, None] == 0 < sizes[1, 1536, None]
+
+
+def test_chosen_pages_go_whole_or_along_the_line(call):  # noqa: F811
+    """No size takes chosen pages in parts of a row: the kernels have no code for it."""
+    call.cache.kv_heads, seen = 1, set()
+    path = C.c_uint32()
+    for page, width, top, seqs, new, heads, cu in itertools.product((32, 1024), (4, 300, 60000), (1, 30, 300, 65536), (1, 3, 190, 5000), (1, 7),
+                                                                    (1, 20, 65536), (None, 4096)):
+        call.cache.page_size, call.batch.table_width, call.batch.table_stride = page, width, width
+        call.batch.n_seqs, call.batch.rows, call.batch.cu = seqs, seqs * new, cu
+        for dtype in (0, 2):
+            assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), dtype, heads, top, C.byref(path)) == 0
+            seen.add(path.value)
+    assert seen == {0, 2}
+    for bad in ((3, 4, 1), (0, 0, 1), (0, 4, 65537)):
+        assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), *bad, C.byref(path)) == ARG
+    assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), 0, 4, 1, None) == ARG
