@@ -8,6 +8,7 @@
 namespace gvdb {
 
 constexpr uint32_t kChooseScores = 15360;  // page scores that a choosing workgroup keeps in LDS: two workgroups a CU
+constexpr uint64_t kScoreBytes = 64ull << 20;  // page scores that a call keeps in scratch: rows are scored and chosen for in groups that fit
 constexpr uint32_t kMaxUnits = 2048;  // sequences or rows that a balanced launch takes
 
 struct KvCache {
@@ -53,8 +54,9 @@ struct AttendArgs {
     // chosen pages
     uint32_t top, first, recent;
     uint32_t score_chunk;      // pages a workgroup scores into `scores`; 0: scored and chosen by one workgroup in LDS
+    uint32_t score_rows;       // rows whose scores `scores` holds at a time
     int32_t* chosen;           // [rows][heads][top]
-    float* scores;             // [rows][heads][table_width]
+    float* scores;             // [score_rows][heads][table_width]
 
     // Pages that hold a query's visible tokens; one beyond the table where the table is too short.
     __host__ __device__ int64_t pages_seen(const KvCache& c, const KvBatch& bt, int64_t limit) const {

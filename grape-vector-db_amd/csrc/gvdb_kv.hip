@@ -1794,21 +1794,26 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
     }
 }
 
-// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds.  One token of 1024 pages,
+// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds; rows [row0, row1) of them.  One token of 1024 pages,
 // 8 heads: 6.5 and 6.5 us, chains of loads; 32 tokens of up to 1563: 16 us, 3 TB/s of bounds, and 10.
 template <int D, int T>
-__global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t chunks) {
+__global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t per, uint32_t chunks, uint32_t row0, uint32_t row1) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t q4 = lane >> 4, n16 = lane & 15u;
     const uint32_t h = blockIdx.x % c.heads, chunk = blockIdx.x / c.heads % chunks;
-    const uint32_t unit = blockIdx.x / c.heads / chunks, b = unit / tok_tiles;
-    int r0, n;
-    seq_rows(bt, b, r0, n);
-    const int64_t before = (int64_t)max(bt.lengths[b], 0) - n + 1;
-    const uint32_t group = a.q_heads / c.heads, width = min(16u, next_pow2(group)), per = 16 / width;
-    for (int t0 = (int)(unit % tok_tiles) * (int)per; t0 < n; t0 += (int)(tok_tiles * per)) {
-        const int toks = min((int)per, n - t0);
-        const int64_t seen = min(a.pages_seen(c, bt, before + t0 + toks - 1), (int64_t)bt.table_width);
+    const uint32_t group = a.q_heads / c.heads, width = min(16u, next_pow2(group));
+    // `per` rows, at most 16 / width: those of one sequence share the bounds that are read
+    int row = (int)(row0 + blockIdx.x / c.heads / chunks * per), toks;
+    const int end = (int)min((uint32_t)row + per, row1);
+    for (; row < end; row += toks) {
+        uint32_t b;
+        toks = 1;
+        if (!a.row_seq(bt, row, b)) continue;
+        int r0, n;
+        seq_rows(bt, b, r0, n);
+        toks = max(min(end, r0 + n) - row, 1);
+        const int64_t limit = (int64_t)max(bt.lengths[b], 0) - n + (row - r0) + toks;  // the last of them sees most
+        const int64_t seen = min(a.pages_seen(c, bt, limit), (int64_t)bt.table_width);
         const int64_t from = (int64_t)chunk * a.score_chunk;
         const int64_t to = chunk + 1 == chunks ? seen : min(seen, from + (int64_t)a.score_chunk);
         const uint32_t my = n16 / width;
@@ -1816,10 +1821,10 @@ __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendA
             const uint32_t gh = g0 + n16 % width;
             ScoreCols<D> col[1];
             col[0].template load<T>(a, (int)my < toks && gh < group,
-                                    (int64_t)(r0 + t0 + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
+                                    (int64_t)(row + (int)my) * a.q.row_stride + (int64_t)(h * group + gh) * a.q.head_stride, q4);
             score_range<D, 1>(c, bt, b, h, col, width, from, to, wave, 4, lane, [&](int, int64_t p, const float(&best)[4]) {
                 if ((int)my >= toks || n16 % width) return;
-                float* out = a.scores + ((uint64_t)(r0 + t0 + (int)my) * c.heads + h) * bt.table_width + p;
+                float* out = a.scores + ((uint64_t)(row - (int)row0 + (int)my) * c.heads + h) * bt.table_width + p;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (p + r < to) out[r] = g0 ? fmaxf(out[r], best[r]) : best[r];
@@ -1828,10 +1833,10 @@ __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendA
     }
 }
 
-__global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch bt, AttendArgs a) {
+__global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch bt, AttendArgs a, uint32_t row0) {
     __shared__ ChooseLds s_choose;
     const uint32_t h = blockIdx.x % c.heads;
-    const int token = (int)(blockIdx.x / c.heads);
+    const int token = (int)(row0 + blockIdx.x / c.heads);
     uint32_t b;
     if (!a.row_seq(bt, token, b)) return;
     int r0, n;
@@ -1842,7 +1847,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch
         for (uint32_t i = threadIdx.x; i < a.top; i += kChooseThreads) out[i] = (int64_t)i < seen ? (int32_t)i : -1;
         return;
     }
-    const float* sc = a.scores + ((uint64_t)token * c.heads + h) * bt.table_width;
+    const float* sc = a.scores + ((uint64_t)(token - (int)row0) * c.heads + h) * bt.table_width;
     const uint32_t width = bt.table_width;
     auto score = [=](uint32_t j) {
         const float x = sc[min(j, width - 1)];
@@ -1945,13 +1950,12 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
     uint32_t per = many ? std::min(groups * per16, kChooseWaves) : per16;
     if (bt.max_new < per) per = next_pow2(bt.max_new);
     while (fused && per > 1 && per * bt.table_width > kChooseScores) per /= 2;
-    const uint32_t chunks = fused ? 1 : (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
-    const uint64_t others = (uint64_t)c.heads * chunks * bt.n_seqs;
-    const uint32_t tok_tiles = capped(((uint64_t)bt.max_new + per - 1) / per, others, 1u << 22);
     const uint64_t blocks = (uint64_t)c.heads * (a.lanes ? a.lanes / 4 : (uint64_t)a.row_tiles * bt.rows);
-    if (!fits(others * tok_tiles, kChooseThreads) || !fits(blocks) || (!fused && !fits((uint64_t)bt.rows * c.heads, kChooseThreads)))
-        return hipErrorInvalidValue;
+    if (!fits(blocks)) return hipErrorInvalidValue;
     if (fused) {
+        const uint64_t others = (uint64_t)c.heads * bt.n_seqs;
+        const uint32_t tok_tiles = capped(((uint64_t)bt.max_new + per - 1) / per, others, 1u << 22);
+        if (!fits(others * tok_tiles, kChooseThreads)) return hipErrorInvalidValue;
         const uint32_t lds = per * bt.table_width * 4;
         auto launch = [&](auto cg) {
             constexpr int CG = decltype(cg)::value;
@@ -1965,10 +1969,16 @@ hipError_t launch_kv_attend_topk(const KvCache& c, const KvBatch& bt, const Atte
         else launch(Const<4>());
         GVDB_LAUNCH_CHECK();
     } else {
-        KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<(uint32_t)(others * tok_tiles), 256, 0, s>>>(c, bt, a, tok_tiles, chunks)));
-        GVDB_LAUNCH_CHECK();
-        k_kv_select<<<bt.rows * c.heads, kChooseThreads, 0, s>>>(c, bt, a);
-        GVDB_LAUNCH_CHECK();
+        const uint32_t chunks = (kv_max_pages(c, bt) + a.score_chunk - 1) / a.score_chunk;
+        if (!fits((uint64_t)((a.score_rows + per - 1) / per) * chunks * c.heads) || !fits((uint64_t)a.score_rows * c.heads, kChooseThreads))
+            return hipErrorInvalidValue;
+        for (uint32_t row0 = 0; row0 < bt.rows; row0 += a.score_rows) {
+            const uint32_t rows = std::min(a.score_rows, bt.rows - row0), tiles = (rows + per - 1) / per;
+            KV_DISPATCH(c.dim, a.q.dtype, (k_kv_score<D, T><<<tiles * chunks * c.heads, 256, 0, s>>>(c, bt, a, per, chunks, row0, row0 + rows)));
+            GVDB_LAUNCH_CHECK();
+            k_kv_select<<<rows * c.heads, kChooseThreads, 0, s>>>(c, bt, a, row0);
+            GVDB_LAUNCH_CHECK();
+        }
     }
     if (a.lanes) {
         KV_DISPATCH(c.dim, a.q.dtype, (k_kv_attend_line<D, T, true><<<(uint32_t)blocks, 256, 0, s>>>(c, bt, a)));

@@ -220,8 +220,11 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
         // 256 pages a workgroup, 64 a wave; 128 where that leaves CUs idle (one sequence of 1024 pages, 8 heads: 31 and 29 us)
         a.score_chunk = !split ? 0 : (uint64_t)bt.rows * c.heads * kv_max_pages(c, bt) < 65536 ? 128 : 256;
         if (split) {
+            // tables of over 15360 pages: a prompt's scores would take gigabytes (2048 tokens, 8 heads, 32768 pages: 2 GiB)
+            const uint64_t row_bytes = (uint64_t)c.heads * bt.table_width * 4;
+            a.score_rows = (uint32_t)std::min<uint64_t>(bt.rows, std::max<uint64_t>(1, kScoreBytes / row_bytes));
             p.scores = at;
-            at += up256((uint64_t)bt.rows * c.heads * bt.table_width * 4);
+            at += up256(a.score_rows * row_bytes);
         }
         p.chosen = at;
         at += up256((uint64_t)bt.rows * c.heads * top * 4);

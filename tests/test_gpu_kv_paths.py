@@ -223,3 +223,55 @@ def test_paths_of_the_other_tests(kv):  # noqa: F811
         table, lens = torch.zeros(seqs, width, dtype=torch.int32, device="cuda"), i32([0] * seqs)
         cu = i32((np.arange(seqs + 1) * new).tolist()) if ragged else None
         assert path(cache, q, table, lens, cu, new, max_len) == want, (dtype, seqs, new)
+
+
+@pytest.mark.parametrize("dtype,Hq,heads,D,new,outside", [("bf16", 3, 1, 64, (700, 1, 1, 600), (2, 3)), ("f16", 20, 1, 128, (1101,), (0, 0)),
+                                                           ("f32", 4, 4, 64, (1,) * 300, (0, 4)), ("bf16", 8, 2, 256, (250, 0, 299), (1, 0))])
+def test_topk_of_long_tables_in_groups_of_rows(kv, dtype, Hq, heads, D, new, outside):  # noqa: F811
+    """More rows than scratch holds the page scores of: groups that end inside a sequence, and inside a workgroup's rows."""
+    page, top, fifty, pages = 32, 6, 50, 16100
+    rng = np.random.default_rng(90)
+    st = Store(kv, 91, dtype, heads, D, page, (page * fifty,))
+    order = rng.integers(0, fifty, (len(new), pages))
+    table = st.table[0, torch.from_numpy(order).cuda()].contiguous()
+    lens = [int(x) for x in rng.integers(pages * page - 200 * page, pages * page, len(new))]
+    q = queries(92, dtype, (sum(outside) + sum(new),), Hq, D).cuda()
+    cu = i32((outside[0] + np.cumsum((0,) + new)).tolist())
+    assert q.shape[0] * heads * pages * 4 > 64 << 20
+    out, chosen = st.cache.attend_topk(q, table, i32(lens), top, first=1, recent=1, cu=cu)
+    got, qd, g = chosen.cpu().numpy(), q.double().cpu().numpy(), Hq // heads
+    bounds = [st.bounds(0, h) for h in range(heads)]
+    row = outside[0]
+    assert (got[:row] == -1).all() and (out[:row] == 0).all()
+    for s, n in enumerate(new):
+        for i in range(n):
+            limit = lens[s] - n + i + 1
+            seen = -(-limit // page)
+            for h in range(heads):
+                # every page scores as the one of the fifty that it is
+                each = scores_of(qd[row, h * g:(h + 1) * g], bounds[h])[order[s, :seen]]
+                each[0] = each[seen - 1] = np.inf
+                assert got[row, h].tolist() == sorted(np.argsort(-each, kind="stable")[:top].tolist()), (s, i, h)
+                if i in (0, n // 2, n - 1) and s < 4:
+                    tokens = (got[row, h][:, None] * page + np.arange(page)).reshape(-1)
+                    tokens = tokens[tokens < limit]
+                    place = order[s][tokens // page] * page + tokens % page
+                    for hq in range(h * g, (h + 1) * g):
+                        o, _, absum, s1 = plain.attend(qd[row, hq], st.k[0][place][:, h], st.v[0][place][:, h], D ** -0.5, np.ones(len(place), bool))
+                        rel = 2 * (D + 8) * 2.0 ** -24 * s1 + (top * page / 32 + 64) * 2.0 ** -23
+                        tol = HALF[dtype] * np.abs(o) + (test_gpu_kv.PROB[dtype] + rel) * (1 + HALF[dtype]) * absum + TINY[dtype]
+                        assert (np.abs(out[row, hq].double().cpu().numpy() - o) <= tol).all(), (s, i, hq)
+            row += 1
+    assert (got[row:] == -1).all() and (out[row:] == 0).all()
+
+
+def scores_of(q, page_bounds):
+    """kv_plain.choose's scores of pages whose bounds are finite."""
+    score = np.full(len(page_bounds), -np.inf)
+    hi, lo = (np.stack([b8[x] for b8, _ in page_bounds]).astype(np.float64) for x in (0, 1))
+    unit = 2.0 ** (np.array([e for _, e in page_bounds], np.float64) - 133)
+    for row in q:
+        a = float(plain.power(np.abs(row).max()))
+        q8 = np.rint(row / 2.0 ** a)
+        score = np.maximum(score, (hi @ np.maximum(q8, 0) + lo @ np.minimum(q8, 0)) * 2.0 ** a * unit)
+    return score

@@ -93,3 +93,17 @@ def test_chosen_pages_go_whole_or_along_the_line(call):  # noqa: F811
     for bad in ((3, 4, 1), (0, 0, 1), (0, 4, 65537)):
         assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), *bad, C.byref(path)) == ARG
     assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), 0, 4, 1, None) == ARG
+
+
+@pytest.mark.parametrize("rows,heads,width", [(2048, 8, 32768), (100000, 8, 15361), (5000, 1, 100000), (3, 4096, 20000), (1, 64, 1 << 20)])
+def test_scratch_of_long_tables_has_a_bound(call, rows, heads, width):  # noqa: F811
+    """Page scores in scratch are those of one row, or 64 MiB; what else there is are the chosen pages and the parts of a join."""
+    call.cache.kv_heads, call.batch.table_width, call.batch.table_stride = heads, width, width
+    call.batch.n_seqs, call.batch.rows, call.batch.max_len = 1, rows, 4096
+    rc, need = call.size(heads=heads, top=4)
+    chosen, join = rows * heads * 4 * 4, 0
+    path = C.c_uint32()
+    for dtype in (0, 2):
+        assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), dtype, heads, 4, C.byref(path)) == 0
+        join |= path.value
+    assert rc == 0 and need <= max(64 << 20, heads * width * 4) + chosen + (32 << 20 if join else 0) + 4096
