@@ -37,7 +37,8 @@ class KvCache:
     [rows, heads, head_dim] in bf16, f16 or f32 with neighbouring channels side by
     side; its rows belong to the sequences by ``cu`` (int32 [sequences + 1]), or
     evenly without it.  ``stream`` (a HIP stream's handle) runs a call there instead of
-    on torch's current stream.  ``max_new`` (most rows of one sequence) and ``max_len`` (the
+    on torch's current stream: the caller orders the two streams; tensors may be dropped as
+    soon as the call returns.  ``max_new`` (most rows of one sequence) and ``max_len`` (the
     largest length) size the launch and change no result.
     """
 
@@ -128,17 +129,26 @@ class KvCache:
     def _stream(self):
         return self._raw_stream(self._index) or None
 
-    def _on(self, stream: int):
-        """Torch's current stream made the given one: what a call allocates belongs to the stream that it runs on."""
+    def _on(self, stream: int, tensors, call):
+        """``call()`` with torch's current stream made the given one.  What it allocates belongs to that stream; what it is given, and
+        the cache, are kept from other use until that stream is through with them, and its results until the caller's is."""
         cuda = self._torch.cuda
-        return cuda.stream(cuda.ExternalStream(stream, device=self.device) if stream else cuda.default_stream(self.device))
+        here = cuda.current_stream(self.device)
+        there = cuda.ExternalStream(stream, device=self.device) if stream else cuda.default_stream(self.device)
+        with cuda.stream(there):
+            result = call()
+        for t in (*tensors, self.pool, self.bounds, self.bound_exps):
+            if t is not None:
+                t.record_stream(there)
+        for t in () if result is None else result if isinstance(result, tuple) else (result,):
+            t.record_stream(here)
+        return result
 
     # -- operators ----------------------------------------------------------
     def append(self, k, v, page_table, lengths, cu=None, max_new: int = 0, stream: Optional[int] = None) -> None:
         """Writes rows ``k`` and ``v`` as tokens ``lengths[s]`` .. of each sequence (``lengths``: tokens before the call)."""
         if stream is not None:
-            with self._on(stream):
-                return self.append(k, v, page_table, lengths, cu, max_new)
+            return self._on(stream, (k, v, page_table, lengths, cu), lambda: self.append(k, v, page_table, lengths, cu, max_new))
         rows = k.shape[0]
         kr = self._rows(k, "k", self.kv_heads, rows)
         vr = self._rows(v, "v", self.kv_heads, rows)
@@ -152,8 +162,8 @@ class KvCache:
         """The stored keys and values of the tokens that an append of ``rows`` rows with the same arguments writes.
         Rows behind the last sequence are left as they were in ``out``, and are 0 without it."""
         if stream is not None:
-            with self._on(stream):
-                return self.read(page_table, lengths, rows, cu, max_new, dtype, out)
+            return self._on(stream, (page_table, lengths, cu, *(out or ())),
+                            lambda: self.read(page_table, lengths, rows, cu, max_new, dtype, out))
         torch, flags = self._torch, 0
         if out is None:
             shape, flags = (rows, self.kv_heads, self.head_dim), _ffi.GVDB_KV_ZERO_REST
@@ -199,8 +209,8 @@ class KvCache:
         sequence's n sees the first ``length - n + i + 1`` tokens.  ``scale``: 1 / sqrt(head_dim) by default; ``lse``
         [rows, heads] float32 takes the logarithm of the softmax's denominator.  A row that sees nothing is 0."""
         if stream is not None:
-            with self._on(stream):
-                return self.attend(q, page_table, lengths, cu, max_new, max_len, scale, causal, out, lse)
+            return self._on(stream, (q, page_table, lengths, cu, out, lse),
+                            lambda: self.attend(q, page_table, lengths, cu, max_new, max_len, scale, causal, out, lse))
         heads, qr, orow, bt, scale, out, scratch, size = self._attend_args(q, page_table, lengths, cu, max_new, max_len, scale, out,
                                                                            lse, 0)
         status = self._lib.gvdb_kv_attend_device(self._ref, bt, qr, heads, scale, 1 if causal else 0, orow, _ffi.ptr(lse),
@@ -216,8 +226,8 @@ class KvCache:
         those whose key bounds promise the largest scores.  Returns ``(out, chosen)``; ``chosen`` is int32 [rows, kv_heads,
         top], positions in the page table in order, -1 behind the last."""
         if stream is not None:
-            with self._on(stream):
-                return self.attend_topk(q, page_table, lengths, top, first, recent, cu, max_new, max_len, scale, out, chosen, lse)
+            return self._on(stream, (q, page_table, lengths, cu, out, chosen, lse),
+                            lambda: self.attend_topk(q, page_table, lengths, top, first, recent, cu, max_new, max_len, scale, out, chosen, lse))
         torch = self._torch
         if top < 1 or first < 0 or recent < 0 or first + recent > top:
             raise InvalidArgument("top is at least 1 and at least first + recent, which are not negative")

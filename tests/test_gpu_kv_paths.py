@@ -275,3 +275,42 @@ def scores_of(q, page_bounds):
         q8 = np.rint(row / 2.0 ** a)
         score = np.maximum(score, (hi @ np.maximum(q8, 0) + lo @ np.minimum(q8, 0)) * 2.0 ** a * unit)
     return score
+
+
+# ---- streams ----------------------------------------------------------------------------------
+def test_tensors_dropped_after_a_call_on_another_stream(kv):  # noqa: F811
+    """The given stream has other work first; what the call was given is dropped and its size asked for again before it runs."""
+    st = Store(kv, 95, "bf16", 2, 128, 64, (3000, 500))
+    q, lens = queries(96, "bf16", (1, 1), 8, 128).cuda(), st.lengths()
+    want, (wk, wc) = st.cache.attend(q, st.table, lens), st.cache.attend_topk(q, st.table, lens, 6)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        given = [q.clone(), st.table.clone(), lens.clone()]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        got = st.cache.attend(*given, stream=side.cuda_stream)
+        gk, gc = st.cache.attend_topk(*given, 6, stream=side.cuda_stream)
+        del given
+        junk = [torch.ones_like(x) for x in (q, st.table, lens) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(gk, wk) and torch.equal(gc, wc)
+        del junk
+
+
+def test_captured_on_a_given_stream(kv):  # noqa: F811
+    st = Store(kv, 97, "bf16", 2, 128, 64, (3000, 500))
+    q, lens = queries(98, "bf16", (1, 1), 8, 128).cuda(), st.lengths()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    st.cache.attend(q, st.table, lens, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = st.cache.attend(q, st.table, lens, stream=side.cuda_stream)
+        pages = st.cache.attend_topk(q, st.table, lens, 6, stream=side.cuda_stream)
+    for i in range(4):
+        q.copy_(queries(99 + i, "bf16", (1, 1), 8, 128))
+        want, (wk, wc) = st.cache.attend(q, st.table, lens), st.cache.attend_topk(q, st.table, lens, 6)
+        out.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(pages[0], wk) and torch.equal(pages[1], wc), i

@@ -3,6 +3,7 @@ import ctypes as C
 import itertools
 
 import pytest
+import torch
 
 from test_kv import ARG, call  # noqa: F401  (call: the fixture)
 
@@ -107,3 +108,80 @@ def test_scratch_of_long_tables_has_a_bound(call, rows, heads, width):  # noqa: 
         assert call.L.gvdb_kv_attend_path(C.byref(call.cache), C.byref(call.batch), dtype, heads, 4, C.byref(path)) == 0
         join |= path.value
     assert rc == 0 and need <= max(64 << 20, heads * width * 4) + chosen + (32 << 20 if join else 0) + 4096
+
+
+# ---- the Python class, on CPU tensors and a library that only says yes ------------------------
+class Kept(torch.Tensor):
+    """A tensor that notes the streams that its memory is kept for."""
+
+    def record_stream(self, stream):
+        self.__dict__.setdefault("streams", []).append(stream)
+
+
+@pytest.fixture()
+def cache(gvdb_mod, monkeypatch):
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from gvdb import _ffi, kv
+
+    now = ["here"]
+
+    @contextmanager
+    def stream(s):
+        before, now[0] = now[0], s
+        yield
+        now[0] = before
+
+    cuda = SimpleNamespace(current_stream=lambda dev: now[0], ExternalStream=lambda s, device: s, default_stream=lambda dev: "default", stream=stream)
+    c = kv.KvCache.__new__(kv.KvCache)
+    c.pool, c.bounds, c.bound_exps = (torch.zeros(n, dtype=torch.uint8).as_subclass(Kept) for n in (34 * 64 * 8, 64, 4))
+    c.n_pages, c.kv_heads, c.head_dim, c.page_size, c.device = 4, 2, 64, 32, torch.device("cpu")
+    c._torch = SimpleNamespace(cuda=cuda, empty=lambda *a, **k: torch.empty(*a, **k).as_subclass(Kept), uint8=torch.uint8, int32=torch.int32,
+                               empty_like=lambda x: torch.empty_like(x).as_subclass(Kept), full=lambda *a, **k: torch.full(*a, **k).as_subclass(Kept),
+                               bfloat16=torch.bfloat16, float32=torch.float32, is_grad_enabled=torch.is_grad_enabled)
+    c._codes = {torch.float32: _ffi.GVDB_F32, torch.float16: _ffi.GVDB_F16, torch.bfloat16: _ffi.GVDB_BF16}
+    c._i32, c._index, c._scale, c._sizes, c._ref = torch.int32, -1, 0.125, {}, None
+    c.ran = []
+    c._raw_stream = lambda index: c.ran.append(now[0])
+
+    class Yes:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    c._lib = Yes()
+    return c
+
+
+def calls(cache):
+    """Every call of the class, and the tensors that it is given."""
+    def t(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(Kept)
+
+    q, k, v, table, lens, cu = t(3, 4, 64), t(3, 2, 64), t(3, 2, 64), t(2, 2, dtype=torch.int32), t(2, dtype=torch.int32), t(3, dtype=torch.int32)
+    out, kv2, lse, chosen = t(3, 4, 64), (t(3, 2, 64), t(3, 2, 64)), t(3, 4), t(3, 2, 2, dtype=torch.int32)
+    return [
+        (lambda **s: cache.append(k, v, table, lens, cu=cu, **s), (k, v, table, lens, cu)),
+        (lambda **s: cache.read(table, lens, 3, cu=cu, **s), (table, lens, cu)),
+        (lambda **s: cache.read(table, lens, 3, cu=cu, out=kv2, **s), (table, lens, cu, *kv2)),
+        (lambda **s: cache.attend(q, table, lens, cu=cu, **s), (q, table, lens, cu)),
+        (lambda **s: cache.attend(q, table, lens, cu=cu, out=out, lse=lse, **s), (q, table, lens, cu, out, lse)),
+        (lambda **s: cache.attend_topk(q, table, lens, 2, cu=cu, **s), (q, table, lens, cu)),
+        (lambda **s: cache.attend_topk(q, table, lens, 2, cu=cu, out=out, chosen=chosen, lse=lse, **s), (q, table, lens, cu, out, chosen, lse)),
+    ]
+
+
+@pytest.mark.parametrize("number", range(7))
+@pytest.mark.parametrize("stream,name", [(4242, 4242), (0, "default")])
+def test_a_call_on_another_stream_keeps_what_it_works_on(cache, number, stream, name):
+    """Dropped tensors would be handed out again on their own stream while the other one still reads or writes them."""
+    run, given = calls(cache)[number]
+    result = run(stream=stream)
+    assert cache.ran == [name]
+    for x in (*given, cache.pool, cache.bounds, cache.bound_exps):
+        assert name in x.streams
+    for x in () if result is None else result if isinstance(result, tuple) else (result,):
+        assert "here" in x.streams
+    run, given = calls(cache)[number]
+    run()  # on the current stream nothing is noted
+    assert cache.ran == [name, "here"] and not any(hasattr(x, "streams") for x in given)
