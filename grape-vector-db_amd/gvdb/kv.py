@@ -39,7 +39,8 @@ class KvCache:
     evenly without it.  ``stream`` (a HIP stream's handle) runs a call there instead of
     on torch's current stream: the caller orders the two streams; tensors may be dropped as
     soon as the call returns.  ``max_new`` (most rows of one sequence) and ``max_len`` (the
-    largest length) size the launch and change no result.
+    largest length) size the launch and change no result.  Nothing here has a gradient: rows
+    that require one are refused where gradients are recorded.
     """
 
     def __init__(self, n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device=None):
@@ -102,6 +103,8 @@ class KvCache:
             raise InvalidArgument(f"{what} is on {t.device}, the cache on {self.device}")
         if stride[2] != 1:
             raise InvalidArgument(f"{what}'s neighbouring channels lie side by side")
+        if t.requires_grad and self._torch.is_grad_enabled():  # its result would silently have none
+            raise InvalidArgument(f"{what} requires a gradient, which a cache in 4 bits does not have: detach it, or call under torch.no_grad()")
         return _ROWS(t.data_ptr(), stride[0], stride[1], code, flags)
 
     def _batch(self, page_table, lengths, cu, rows: int, max_new: int, max_len: int):

@@ -185,3 +185,24 @@ def test_a_call_on_another_stream_keeps_what_it_works_on(cache, number, stream, 
     run, given = calls(cache)[number]
     run()  # on the current stream nothing is noted
     assert cache.ran == [name, "here"] and not any(hasattr(x, "streams") for x in given)
+
+
+def test_rows_that_require_a_gradient_are_refused(cache):
+    """There is none to give: without a refusal training would go on with what the cache answered as a constant."""
+    from gvdb import InvalidArgument
+
+    table, lens = torch.zeros(2, 2, dtype=torch.int32).as_subclass(Kept), torch.zeros(2, dtype=torch.int32).as_subclass(Kept)
+    q, kv = torch.zeros(2, 4, 64).as_subclass(Kept), torch.zeros(2, 2, 64).as_subclass(Kept)
+    leaf, leaf_kv = q.clone().requires_grad_(), kv.clone().requires_grad_()
+    for rows, other in ((leaf, leaf_kv), (leaf * 2, leaf_kv.transpose(0, 1).contiguous().transpose(0, 1))):
+        tries = (lambda: cache.append(other, kv, table, lens), lambda: cache.append(kv, other, table, lens),
+                 lambda: cache.read(table, lens, 2, out=(kv, other)), lambda: cache.attend(rows, table, lens),
+                 lambda: cache.attend(q, table, lens, out=rows), lambda: cache.attend_topk(rows, table, lens, 2),
+                 lambda: cache.attend(rows, table, lens, stream=7))
+        for call_it in tries:
+            with pytest.raises(InvalidArgument, match="gradient"):
+                call_it()
+            with torch.no_grad():
+                call_it()
+        cache.attend(rows.detach(), table, lens)
+    assert not cache.attend(q, table, lens).requires_grad
