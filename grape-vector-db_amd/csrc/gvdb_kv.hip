@@ -410,8 +410,9 @@ __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows
             const uint32_t e = any ? 255u : min(max((amax + 0x1FFFFu) >> 23, 7u), 254u);
             const float up = bits_f32((260u - min(e, 254u)) << 23);  // 2^(133 - e)
             int8_t* q = c.bounds + ((uint64_t)page * c.heads + h) * (2 * D);
-            q[d] = any ? (int8_t)0 : (int8_t)ceilf(h1 * up);
-            q[D + d] = any ? (int8_t)0 : (int8_t)floorf(l1 * up);
+            // a product too small for a float is 0, which bounds nothing: outward of it is a step
+            q[d] = any ? (int8_t)0 : (int8_t)fmaxf(ceilf(h1 * up), h1 > 0.f ? 1.f : -127.f);
+            q[D + d] = any ? (int8_t)0 : (int8_t)fminf(floorf(l1 * up), l1 < 0.f ? -1.f : 127.f);
             if (d == 0) c.bound_exps[(uint64_t)page * c.heads + h] = (uint8_t)e;
         }
         __syncthreads();

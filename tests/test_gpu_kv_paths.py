@@ -314,3 +314,44 @@ def test_captured_on_a_given_stream(kv):  # noqa: F811
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(pages[0], wk) and torch.equal(pages[1], wc), i
+
+
+# ---- append, read: the ends of the 16-bit types -----------------------------------------------
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_append_of_subnormal_and_extreme_16_bit_values(kv, dtype, D):  # noqa: F811
+    """Every bit pattern of the type in groups of its own size and beside larger and smaller ones, infinities and NaN among them."""
+    rng = np.random.default_rng(110)
+    bits = np.arange(1 << 16, dtype=np.uint32).astype(np.uint16)
+    width = 10 if dtype == "f16" else 7
+    exps = (bits >> width) & ((1 << (15 - width)) - 1)
+    groups = [rng.permutation(bits[exps == e])[:2048].reshape(-1, 32) for e in range(exps.max() + 1) if (exps == e).sum() >= 32]
+    small = bits[exps <= 1]
+    groups += [rng.choice(small, (400, 32)), rng.choice(bits[exps < exps.max()], (400, 32))]
+    mixed = rng.choice(small, (60, 32))
+    mixed[:, 5] = rng.choice(bits[(exps > 1) & (exps < 12)], 60)
+    few = np.zeros((40, 32), np.uint16)  # almost nothing: a group's only value is one of the smallest
+    few[:, 9] = np.r_[np.arange(1, 31), 0x8000 + np.arange(1, 11)]
+    x = np.concatenate(groups + [mixed, few])
+    x = x[:len(x) // (D // 32) * (D // 32)].reshape(-1, 1, D)
+    t = torch.from_numpy(x.view(np.int16)).view(DT[dtype])
+    n, page = len(x), 64
+    need = -(-n // page)
+    cache, table = kv.KvCache(need, 1, D, page), torch.arange(need, dtype=torch.int32, device="cuda")[None]
+    cache.append(t.cuda(), t.flip(0).cuda(), table, i32([0]))
+    k, v = cache.read(table, i32([0]), n, dtype=torch.float32)
+    want = plain.stored(t.double().numpy())
+    assert np.array_equal(k.double().cpu().numpy(), want, equal_nan=True)
+    assert np.array_equal(v.flip(0).double().cpu().numpy(), want, equal_nan=True)
+    assert np.isnan(want).any() and (np.abs(want[np.isfinite(want)]) > 0).any()
+    b8, be = cache.bounds.cpu().numpy(), cache.bound_exps.cpu().numpy()
+    for j in range(need):
+        rows = want[j * page:(j + 1) * page, 0]
+        b, e = plain.bounds(rows)
+        e = 7 if not rows.any() else e  # nothing but zeros: the smallest power that there is (frexp(0) says 2^0)
+        assert be[j, 0] == e and np.array_equal(b8[j, 0], b), j
+    # read back in any type: rounded once
+    for other in DT.values():
+        k, _ = cache.read(table, i32([0]), n, dtype=other)
+        finite = torch.from_numpy(want).float()  # exact: a code has two bits, its power of two is 2^-125 at least
+        assert torch.equal(k.cpu().nan_to_num(7.0, posinf=8.0, neginf=-8.0), finite.to(other).nan_to_num(7.0, posinf=8.0, neginf=-8.0))
