@@ -259,7 +259,8 @@ gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const
     if (gvdb_status s = take_batch(batch, call.c, call.bt)) return s;
     if (choose && top == 0) return invalid("token cache: top is at least 1");
     if (choose && (uint64_t)first + recent > top) return invalid("token cache: first + recent is at most top");
-    if (!std::isfinite(scale)) return invalid("token cache: scale is not finite");
+    const float base2 = std::fabs(scale) * 1.4426950408889634f;
+    if (!std::isfinite(base2)) return invalid("token cache: scale is not finite, or is not times log2(e)");
     if (call.bt.rows == 0) return GVDB_OK;
     Plan p;
     KvRows qr, orow;
@@ -274,8 +275,8 @@ gvdb_status attend(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const
     AttendArgs& a = p.a;
     uint8_t* base = (uint8_t*)scratch;
     a.lse = lse;
-    // a scale of 0 (every token alike) is one that no finite score notices: -inf times it has to stay -inf
-    a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 0x1p-120f);
+    // a scale of 0 (every token alike) is the least that there is, which no finite score notices: -inf times it has to stay -inf
+    a.scale_log2 = std::max(base2, 0x1p-149f);
     a.negate = scale < 0;
     a.causal = causal != 0;
     a.first = first;

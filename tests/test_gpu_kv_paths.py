@@ -355,3 +355,21 @@ def test_append_of_subnormal_and_extreme_16_bit_values(kv, dtype, D):  # noqa: F
         k, _ = cache.read(table, i32([0]), n, dtype=other)
         finite = torch.from_numpy(want).float()  # exact: a code has two bits, its power of two is 2^-125 at least
         assert torch.equal(k.cpu().nan_to_num(7.0, posinf=8.0, neginf=-8.0), finite.to(other).nan_to_num(7.0, posinf=8.0, neginf=-8.0))
+
+
+@pytest.mark.parametrize("dtype,Hq,D,new,n", [("f32", 2, 64, 3, 90), ("bf16", 2, 128, 1, 90), ("bf16", 8, 64, 128, 150), ("f32", 1, 256, 1, 3000)])
+def test_a_scale_of_nothing_weighs_all_alike(kv, dtype, Hq, D, new, n):  # noqa: F811
+    """Whatever the scores are that it is multiplied with; and a scale that is next to nothing is what it is."""
+    copies = 96 if new == 128 else 1
+    st = Store(kv, 120, dtype, 1, D, 64, (n,))
+    big = torch.randn(n, 1, D, generator=torch.Generator().manual_seed(1)) * 1e17
+    big = big.to(DT[dtype])
+    v = torch.randn(n, 1, D, generator=torch.Generator().manual_seed(2)).to(DT[dtype])
+    st.cache.append(big.cuda(), v.cuda(), st.table, i32([0]))
+    st.k[0], st.v[0] = plain.stored(big.double().numpy()), plain.stored(v.double().numpy())
+    q = (queries(121, dtype, (new,), Hq, D).float() * 1e18).to(DT[dtype])
+    table, lens = st.table.repeat(copies, 1), i32([n] * copies)
+    for scale in (0.0, -0.0, 1e-40, 3e-37):
+        out = st.cache.attend(q.repeat(copies, 1, 1).cuda(), table, lens, causal=False, scale=scale)
+        assert new != 128 or path(st.cache, q.repeat(copies, 1, 1), table, lens) == ROWS
+        check_attend(st, q[:4], (min(new, 4),), out[:4], causal=False, scale=float(np.float32(scale)))

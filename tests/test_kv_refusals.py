@@ -206,3 +206,11 @@ def test_rows_that_require_a_gradient_are_refused(cache):
                 call_it()
         cache.attend(rows.detach(), table, lens)
     assert not cache.attend(q, table, lens).requires_grad
+
+
+def test_scales_beyond_the_range_of_floats(call):  # noqa: F811
+    """In units of base 2, in which the kernels have it, a scale is finite too."""
+    call.batch.table_width = call.batch.table_stride = 5000
+    need = call.size()[1]
+    for scale, why in ((2.3e38, "scratch"), (-2.3e38, "scratch"), (2.4e38, "scale"), (-3.4e38, "scale")):
+        assert call.attend(scale=scale, size=need - 1) == ARG and why in call.why(), scale
