@@ -1454,6 +1454,7 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
 // Score of a page for a query head: 2^(a + b) * sum_d max(q8_d, 0) hi_d + min(q8_d, 0) lo_d with q8 = rint(q / 2^a) and the
 // page's bounds hi, lo in units of 2^b.  The sum is a product of whole numbers over 2 D channels: v_mfma_i32_16x16x64_i8,
 // exact in any order.  A wave scores 16 pages for 16 columns: `width` columns (a power of two) a token, the group's heads.
+constexpr float kNotFinite = INFINITY;  // score of a page that holds what is not finite, or is not there: over all others, which end at the largest float
 template <int D>
 struct ScoreCols {  // this lane's column: channels k * 64 + q4 * 16 .. + 16 in 8 bits
     u4 pos[D / 64], neg[D / 64];
@@ -1534,7 +1535,7 @@ __device__ __forceinline__ void score_pages(const u4 (&pb)[D / 32], uint32_t e, 
     if (width > 4) row_max_step<0x141>(best);
     if (width > 8) row_max_step<0x140>(best);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) best[r] = be[r] == 255u ? 3.402823466e38f : best[r];
+    for (int r = 0; r < 4; ++r) best[r] = be[r] == 255u ? kNotFinite : fminf(best[r], 3.402823466e38f);
 }
 
 // Scores of pages [from, to) for CG times 16 / width tokens, 64 pages a wave at a time, all their bounds in flight at once (D = 256, and
@@ -1779,7 +1780,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
             // a page beyond the table is the last: it is among the recent ones, or scores as one that is not there
             auto score = [=](uint32_t j) {
                 const float x = sc[min(j, in_lds - 1)];
-                return j < in_lds ? x : 3.402823466e38f;
+                return j < in_lds ? x : kNotFinite;
             };
             if (mine > (int64_t)a.top && toks == 1) {
                 choose_pages<kChooseWaves>(a, score, (uint32_t)mine, out, s_choose, wave, lane);
@@ -1852,7 +1853,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_select(KvCache c, KvBatch
     const uint32_t width = bt.table_width;
     auto score = [=](uint32_t j) {
         const float x = sc[min(j, width - 1)];
-        return j < width ? x : 3.402823466e38f;
+        return j < width ? x : kNotFinite;
     };
     choose_pages<kChooseWaves>(a, score, (uint32_t)seen, out, s_choose,
                                __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threadIdx.x & 63u);

@@ -373,3 +373,18 @@ def test_a_scale_of_nothing_weighs_all_alike(kv, dtype, Hq, D, new, n):  # noqa:
         out = st.cache.attend(q.repeat(copies, 1, 1).cuda(), table, lens, causal=False, scale=scale)
         assert new != 128 or path(st.cache, q.repeat(copies, 1, 1), table, lens) == ROWS
         check_attend(st, q[:4], (min(new, 4),), out[:4], causal=False, scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("pages,new,max_len", [(60, 1, 0), (60, 9, 0), (700, 1, 0)])
+def test_topk_takes_what_is_not_finite_before_scores_that_overflow(kv, pages, new, max_len):  # noqa: F811
+    """Scores beyond the range of 32 bits are equal, and less than a page that holds what is not finite, or is not there."""
+    D, page = 64, 32
+    cache = kv.KvCache(pages, 1, D, page)
+    k = torch.full((pages * page, 1, D), 1e14, device="cuda")
+    k[(pages - 8) * page + 3, 0, 7] = float("nan")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cache.append(k, k, table, i32([0]))
+    table[0, pages - 5] = -1
+    q = torch.full((new, 2, D), 1e30, device="cuda")
+    _, chosen = cache.attend_topk(q, table, i32([pages * page]), 6, first=0, recent=1, max_len=max_len)
+    assert chosen[:, 0].tolist() == [[0, 1, 2, pages - 8, pages - 5, pages - 1]] * new
