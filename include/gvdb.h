@@ -621,11 +621,14 @@ gvdb_status gvdb_kv_attend_path(const gvdb_kv_cache* cache, const gvdb_kv_batch*
  * reads key/value head h / (q_heads / kv_heads).  A row that sees no token is 0
  * (lse: -inf).  lse: device [rows][q_heads] f32, the natural logarithm of the
  * softmax's denominator, or NULL.  q and out: one type, q_heads heads; out's
- * rows must not overlap, and out may be q itself.  A row of q that holds an
- * infinity or a NaN is NaN where it sees a token, and spoils no other row.
- * Sums and statistics are kept in 32 bits; keys, values and queries enter the
- * products exactly, the probabilities in 16 bits for bf16 and f16 rows and in
- * 24 for f32, whatever the hints and the other sequences of the batch are. */
+ * rows must not overlap, and out may be q itself (or share no memory with it).
+ * A row of q that holds an infinity or a NaN is NaN where it sees a token, and
+ * spoils no other row.  Keys, values and queries enter the products exactly, the
+ * probabilities in 16 bits for bf16 and f16 rows and in 24 for f32, whatever the
+ * hints and the other sequences of the batch are.  Sums and statistics are kept
+ * in 32 bits, and values are summed before they are divided by the denominator:
+ * a score q . k over 2^128 makes its row NaN, one below -2^128 is not seen, and
+ * values over 2^120 divided by the number of tokens may make a row infinite. */
 gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
                                   uint32_t q_heads, float scale, int32_t causal, const gvdb_kv_rows* out, float* lse,
                                   void* scratch, uint64_t scratch_bytes, void* stream);
