@@ -388,3 +388,72 @@ def test_topk_takes_what_is_not_finite_before_scores_that_overflow(kv, pages, ne
     q = torch.full((new, 2, D), 1e30, device="cuda")
     _, chosen = cache.attend_topk(q, table, i32([pages * page]), 6, first=0, recent=1, max_len=max_len)
     assert chosen[:, 0].tolist() == [[0, 1, 2, pages - 8, pages - 5, pages - 1]] * new
+
+
+# ---- calls that are allowed and rarely made ---------------------------------------------------
+@pytest.mark.parametrize("dtype,Hq,heads,D,page", [("bf16", 32, 1, 64, 64), ("f16", 32, 2, 128, 32), ("bf16", 32, 1, 256, 64)])
+def test_what_is_masked_in_parts_of_rows_may_hold_anything(kv, dtype, Hq, heads, D, page):  # noqa: F811
+    for poison in (float("nan"), float("inf"), -float("inf")):
+        c = Crowd(kv, ROW_PARTS, 130, dtype, Hq, heads, D, page, (150, 40), (80, 9), 1)
+        st = c.st
+        k = torch.from_numpy(np.random.default_rng(1).standard_normal((4, heads, D))).to(DT[dtype]).cuda()
+        v = k.clone()
+        v[1, :, 40] = poison   # token 121: a value, channels 32 .. 63
+        k[3, :, 7] = poison    # token 123: a key
+        st.cache.append(k, v, st.table[:1], i32([120]))
+        st.k[0][120:124], st.v[0][120:124] = plain.stored(k.double().cpu().numpy()), plain.stored(v.double().cpu().numpy())
+        c.q[5, 1, 0] = poison
+        lse = torch.empty(c.q.shape[:2], device="cuda")
+        out = c.attend(lse=lse)
+        want = np.zeros((89, Hq, D), bool)
+        want[51:80, :, 32:64] = True    # row i of the 80 is token 70 + i
+        want[53:80] = True
+        want[5, 1] = True
+        assert np.array_equal(torch.isnan(out).cpu().numpy(), want)
+        c.one = c.q
+        c.check(out, lse, skip={(r, h) for r in range(51, 80) for h in range(Hq)} | {(5, 1)})
+
+
+def test_calls_without_rows(kv):  # noqa: F811
+    st = Store(kv, 131, "bf16", 2, 64, 32, (40, 9))
+    before = [x.clone() for x in (st.cache.pool, st.cache.bounds, st.cache.bound_exps)]
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for table, lens, cu in ((st.table, st.lengths(), None), (st.table, st.lengths(), i32([0, 0, 0])), (st.table[:0], i32([]), None)):
+        st.cache.append(q[:, :2], q[:, :2], table, lens, cu=cu)
+        assert st.cache.attend(q, table, lens, cu=cu).shape == (0, 4, 64)
+        out, chosen = st.cache.attend_topk(q, table, lens, 3, cu=cu)
+        assert out.shape == (0, 4, 64) and chosen.shape == (0, 2, 3)
+        assert all(x.shape == (0, 2, 64) for x in st.cache.read(table, lens, 0, cu=cu))
+    assert all(torch.equal(a, b) for a, b in zip(before, (st.cache.pool, st.cache.bounds, st.cache.bound_exps)))
+
+
+@pytest.mark.parametrize("Hq,heads,D,dtype", [(2048, 1, 64, "bf16"), (333, 1, 256, "f32"), (300, 300, 64, "f16")])
+def test_many_heads(kv, Hq, heads, D, dtype):  # noqa: F811
+    st = Store(kv, 132, dtype, heads, D, 32, (200, 70))
+    q, cu = queries(133, dtype, (2, 1), Hq, D).cuda(), i32([0, 2, 3])
+    lse = torch.empty(3, Hq, device="cuda")
+    skip = {(i, h) for i in range(3) for h in range(Hq) if h % 37}
+    check_attend(st, q, (2, 1), st.cache.attend(q, st.table, st.lengths(), cu=cu, lse=lse), lse, skip=skip)
+    out, chosen = st.cache.attend_topk(q, st.table, st.lengths(), 3, cu=cu, lse=lse)
+    check_attend(st, q, (2, 1), out, lse, chosen=chosen.cpu().numpy(), skip=skip)
+
+
+def test_row_bounds_and_lengths_that_make_no_sense(kv):  # noqa: F811
+    """They lead nowhere outside the tensors, the table and the pool; what they leave in the cache is not checked."""
+    for bad in ([0, 3, 1], [-5, 100, 2], [3, 2, 1], [2 ** 31 - 1, 0, 5], [5, -2 ** 31, 5]):
+        st = Store(kv, 134, "bf16", 2, 64, 32, (40, 9))
+        q, cu = queries(135, "bf16", (5,), 4, 64).cuda(), i32(bad)
+        guard = torch.full((7, 4, 64), 3.0, dtype=q.dtype, device="cuda")
+        st.cache.attend(q, st.table, st.lengths(), cu=cu, out=guard[1:6])
+        st.cache.attend_topk(q, st.table, st.lengths(), 2, cu=cu, out=guard[1:6])
+        st.cache.read(st.table, st.zeros(), 5, cu=cu)
+        st.cache.append(q[:, :2], q[:, :2], st.table, st.zeros(), cu=cu)
+        torch.cuda.synchronize()
+        assert (guard[0] == 3).all() and (guard[6] == 3).all()
+    for lens, nan in (((-5, 2 ** 31 - 1), [False, True]), ((-2 ** 31, 0), [False, False])):
+        st = Store(kv, 136, "bf16", 2, 64, 32, (40, 9))
+        q, k = queries(137, "bf16", (2,), 4, 64).cuda(), st.cache.pool.clone()
+        for out in (st.cache.attend(q, st.table, i32(lens)), st.cache.attend_topk(q, st.table, i32(lens), 2)[0]):
+            assert [bool(torch.isnan(x).all()) for x in out] == nan and bool((out[0] == 0).all())
+        st.cache.append(q[:, :2], q[:, :2], st.table[:, :1].contiguous(), i32([2 ** 31 - 1, 33]))  # behind the table: skipped
+        assert torch.equal(k, st.cache.pool)
