@@ -39,8 +39,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kLowest = -3e38f;  // running maximum before the first key: finite, so that -inf - m is -inf and not NaN
 // Pieces of 8 bits that a type's values are split into for the products.
 constexpr int pieces(int dtype) { return dtype == GVDB_BF16 ? 1 : dtype == GVDB_F16 ? 2 : 3; }
-// Pieces of a probability, on every path alike: 16 bits for rows of 16 bits, 24 for those of 32.  With one piece for
-// bf16 rows half of an output's error would be the probabilities', and the size of a launch would decide how many bits a row gets.
+// Pieces of a probability, on every path alike: 16 bits for rows of 16 bits, 24 for those of 32.  Rows of 16 bits are as far from 64 bits
+// as with 32 (0.0017 relative in bf16, 0.00021 in f16, an output's own rounding); with one piece for bf16 rows 0.0023 by 128 rows, and
+// the size of a launch would decide how many bits a row gets.
 template <int NP>
 constexpr int kProbPieces = NP < 2 ? 2 : NP;
 // The value, as one that the compiler knows nothing of: what is reckoned from it in a branch that is seldom taken stays in
@@ -297,9 +298,10 @@ struct Raw8 {
 
 // ---- append -----------------------------------------------------------------------------
 // One workgroup a touched page, head and part (keys, values).  D / 8 threads take a token, eight channels each; four neighbours
-// share a scale.  Four passes' loads are in flight at once.  Bound by the reads of k and v where there are many tokens (16384 tokens
-// of 8 heads of 128 channels, bf16: 25 us, 3.4 TB/s read and written), and by its chain of loads (length, page, rows and the codes
-// that the page's bounds go over) where there is one: 64 sequences' next tokens 8 us.
+// share a scale.  Four passes' loads are in flight at once.  Where there are many tokens (16384 of 8 heads of 128 channels, bf16: 28 us,
+// 3.0 TB/s read and written) bound by the reads of k and v and by what lies between them: nothing is in flight while a page's bounds are
+// reckoned.  Where there is one, by its chain of loads (length, page, rows and the codes that the page's bounds go over): 64 sequences'
+// next tokens 8 us.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows k, KvRows v, uint32_t slots) {
     constexpr uint32_t TPT = D / 8;       // threads a token
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvCache c, KvBatch bt, KvRows
 
 // ---- read -------------------------------------------------------------------------------
 // A thread takes eight channels of one token and head, keys and values; a workgroup several tokens of one head, whose codes lie
-// side by side.  Bound by what it writes (the same 16384 tokens: 17.5 us, 4.9 TB/s).
+// side by side.  Bound by what it writes (the same 16384 tokens: 18.5 us, 4.6 TB/s).
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_read(KvCache c, KvBatch bt, KvRows k, KvRows v) {
     constexpr uint32_t TPT = D / 8;
@@ -918,9 +920,9 @@ __device__ __forceinline__ void write_wave(Rows<D, NP>& w, const Job<CHOSEN>& j,
 // A workgroup takes 16 query rows of a unit and key head and one split of its tiles; its four waves take steps of them in
 // turn, one step's loads in flight while another is worked on, and join their parts through LDS.  With one query token a
 // sequence each cached byte is read once: 34 D / 32 bytes a token and head bound it where there are many (32 sequences of 32 pages:
-// 18.5 us).  One sequence of 768 tokens takes 9 us, of which its 24 tiles are 4; the rest is the chain of
+// 20 us).  One sequence of 768 tokens takes 9 us, of which its 24 tiles are 4; the rest is the chain of
 // loads before the first product (length, table, tiles), the join and the launch.
-// 384 tokens' own 40 pages of 32, 4 heads: 47 us, 5.7 TB/s out of the caches and three quarters of the cycles in vector instructions.
+// 384 tokens' own 40 pages of 32, 4 heads: 46 us, 5.8 TB/s out of the caches and three quarters of the cycles in vector instructions.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 : 3) void k_kv_attend(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T);
@@ -972,7 +974,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 && T == GVDB_F32 ? 2 :
 // wave takes whole is written at once; the others' parts go to slot w + u (w and u only ever grow along the line: no two
 // parts share one) and are joined by k_kv_combine.  Waves never wait for one another, and loads run on over the borders
 // of units, the next unit's queries among them.  Bound by the reads: 4 sequences of 262144 tokens, 8 heads of 128 channels, 205 us with
-// the join, 5.6 TB/s; 64 of up to 10000, 57 us, 4.1 TB/s, of which the join is 5.
+// the join, 5.6 TB/s; 64 of up to 10000, 57 us, 4.1 TB/s, of which the join is 6.
 template <int D, int T, bool CHOSEN>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_kv_attend_line(KvCache c, KvBatch bt, AttendArgs a) {
     constexpr int NP = pieces(T);
@@ -1064,9 +1066,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void k_kv_att
 // into LDS (two buffers, one barrier a step), as [8 tokens][channels][16 bytes], the operand as it is read.
 // A row of keys stands for token t(row) with bits 2 and 3 exchanged, so that S^T leaves a lane with eight neighbouring
 // tokens of its query row, which O^T = V^T P^T takes as they are.  Channel j of sixteenth l lies at row 16 j + l of V^T.
-// Bound by the vector instructions that expand keys and reckon probabilities: 2048 tokens of 2 sequences over 10000, 32 heads on 8 of
-// 128 channels, 839 us, 720 TFLOP/s (with probabilities of 8 bits, whose products are half as many, 639 us); two workgroups a CU, all
-// that the registers hold, overlap them and the products no further.
+// Bound by the vector instructions that expand keys and reckon probabilities and their pieces: 2048 tokens of 2 sequences over 10000, 32
+// heads on 8 of 128 channels, 837 us, 720 TFLOP/s (with probabilities of 8 bits 639 us); vector instructions issue in 66 % of the cycles,
+// the matrix units are busy in 49 %, and two workgroups a CU, all that the registers hold, overlap them no further.
 template <int D, int NP>
 struct Rows32 {
     u4 qf[NP][D / 16];  // query pieces: lane 32 i + n has row n, channels [i D/2, (i+1) D/2)
@@ -1707,7 +1709,7 @@ __device__ __forceinline__ void choose_pages(const AttendArgs& a, Scores sc, uin
 // One workgroup: the pages of `per` tokens of a sequence (at most CG times 16 / width) and one key head, scored into LDS and chosen
 // there.  The tokens share the bounds that it reads, 2 D + 1 bytes a page.  CG > 1: a wave quantises sixteen columns for all of them,
 // and hands them on through LDS; with every wave at all of them, and the loop over pages unrolled, it waited for its own code.
-// 384 tokens, 4 heads, 1024 pages: 35 us (45 before; 67 by one sixteen columns a workgroup), about a third each for the prologue, the
+// 384 tokens, 4 heads, 1024 pages: 36 us (45 before; 67 by one sixteen columns a workgroup), about a third each for the prologue, the
 // scores and the choice, none of them near a rate of the card: 192 workgroups, a chain of short phases.  3800 pages: 95 us.
 template <int D, int T, int CG>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch bt, AttendArgs a, uint32_t tok_tiles, uint32_t per) {
@@ -1797,7 +1799,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
 }
 
 // The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds; rows [row0, row1) of them.  One token of 1024 pages,
-// 8 heads: 6.5 and 6.5 us, chains of loads; 32 tokens of up to 1563: 16 us, 3 TB/s of bounds, and 10.
+// 8 heads: 7 us and 6 to 10, chains of loads; 32 tokens of up to 1563: 17 us, 2.8 TB/s of bounds, and 10.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t per, uint32_t chunks, uint32_t row0, uint32_t row1) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -150,9 +150,9 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
     // with three.
     const uint64_t slots = c.dim == 256 ? 256 : c.dim == 128 ? 512 : 768;
     // Workgroups of 128 rows share the values' expansion, and run in rounds.  A round of m workgroups a CU takes about (m + 1) / 2 times
-    // what one of a single one does, 8 tiles' time before its first tile, and a join as much again; in units of half a tile, 0.42 us, with
-    // the number of parts that takes least (2 sequences of 300 tokens over 5000: 3 parts 116 us, 5 131, 1 180; 6 of 256 over 1500: 1 67,
-    // 3 93).
+    // what one of a single one does, 8 tiles' time before its first tile, and a join as much again; in units of half a tile (0.36 us
+    // at 64 channels, 0.53 at 128, 0.8 at 256), with the number of parts that takes least (2 sequences of 300 tokens over 5000: 3 parts
+    // 109 us, 5 125, 1 160; 6 of 256 over 1500: 1 82, 3 106).
     const uint64_t busy128 = busy_of(128, units0 * c.heads * ((rows_each + 127) / 128));
     uint64_t time128 = ~0ull, parts128 = 1;
     for (uint64_t k = 1; k <= std::max<uint64_t>(1, tiles / 16) && k <= 64; ++k) {
@@ -161,8 +161,8 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
         if (time < time128) time128 = time, parts128 = k;
     }
     // By 16 rows the card does 800 tiles (64 channels: 1000) in one of these units, 5 go by before a workgroup's first, and a join where
-    // they are too few to go whole.  16 sequences of 64 tokens over 900, 4 heads a group: 36 us by 128 rows, 27 by 16; 64 over 300 57 and
-    // 90; 2 over 16000 48 and 56; 2 of 2048 over 10000, 8 heads: 630 and 1110.  In 32 bits the pieces do not fit the registers: 130 and
+    // they are too few to go whole.  16 sequences of 64 tokens over 900, 4 heads a group: 41 us by 128 rows, 27 by 16; 64 over 300 58 and
+    // 90; 2 over 16000 53 and 56; 2 of 2048 over 10000, 8 heads: 837 and 1156.  In 32 bits the pieces do not fit the registers: 130 and
     // 117 us at 512 rows.
     const uint64_t busy16 = busy_of(16, units0 * c.heads * ((rows_each + 15) / 16));
     a.many = !top && dtype != GVDB_F32 && rows_each >= 128 && time128 < 5 + busy16 * (tiles + 5) / (c.dim == 64 ? 1000 : 800) + (busy16 < 512 ? 14 : 0);
@@ -200,8 +200,8 @@ gvdb_status plan_attend(const KvCache& c, const KvBatch& bt, uint32_t dtype, uin
             a.chunk = (uint32_t)((tiles + a.splits - 1) / a.splits + 1) / 2 * 2;
             a.splits = (uint32_t)((tiles + a.chunk - 1) / a.chunk);
         } else {
-            // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 333 us,
-            // for 1024 of them 354, for 512 432), or 2560 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
+            // parts for 2048 workgroups of 128 rows, of which about a third find keys (2 sequences of up to 500 tokens over 30000: 421 us,
+            // for 1024 of them 447, for 512 525), or 2560 of 16 rows (5 tokens of 32 sequences over up to 20000: 81 us, for 1536 85, for
             // 768 121).  Of 16 tiles at least, for 128 rows; of 16 rows a part's time grows with its tiles and the join's with the parts,
             // so of the square root of all tiles (best of 6 .. 32: 94 tiles 8 to 12, 250 12 to 16, 625 24, 938 32)
             const uint64_t parts = a.many ? 2048 : 2560, least = a.many ? 16 : std::max<uint64_t>(8, (uint64_t)std::sqrt((double)tiles));
