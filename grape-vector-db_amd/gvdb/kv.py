@@ -143,7 +143,7 @@ class KvCache:
         for t in (*tensors, self.pool, self.bounds, self.bound_exps):
             if t is not None:
                 t.record_stream(there)
-        for t in () if result is None else result if isinstance(result, tuple) else (result,):
+        for t in () if result is None else result if isinstance(result, (tuple, list)) else (result,):
             t.record_stream(here)
         return result
 
@@ -165,7 +165,7 @@ class KvCache:
         """The stored keys and values of the tokens that an append of ``rows`` rows with the same arguments writes.
         Rows behind the last sequence are left as they were in ``out``, and are 0 without it."""
         if stream is not None:
-            return self._on(stream, (page_table, lengths, cu, *(out or ())),
+            return self._on(stream, (page_table, lengths, cu, *(() if out is None else (out[0], out[1]))),
                             lambda: self.read(page_table, lengths, rows, cu, max_new, dtype, out))
         torch, flags = self._torch, 0
         if out is None:

@@ -214,3 +214,12 @@ def test_scales_beyond_the_range_of_floats(call):  # noqa: F811
     need = call.size()[1]
     for scale, why in ((2.3e38, "scratch"), (-2.3e38, "scratch"), (2.4e38, "scale"), (-3.4e38, "scale")):
         assert call.attend(scale=scale, size=need - 1) == ARG and why in call.why(), scale
+
+
+@pytest.mark.parametrize("kind", ["tuple", "list", "stacked"])
+def test_outputs_of_read_in_any_pair(cache, kind):
+    table, lens = (torch.zeros(*s, dtype=torch.int32).as_subclass(Kept) for s in ((2, 2), (2,)))
+    both = torch.zeros(2, 3, 2, 64).as_subclass(Kept)
+    out = both if kind == "stacked" else (tuple if kind == "tuple" else list)(x.clone().as_subclass(Kept) for x in both)
+    for stream in (None, 4242):
+        assert cache.read(table, lens, 3, cu=torch.zeros(3, dtype=torch.int32).as_subclass(Kept), out=out, stream=stream) is out
