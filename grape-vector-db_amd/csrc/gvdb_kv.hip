@@ -1456,7 +1456,8 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
 // Score of a page for a query head: 2^(a + b) * sum_d max(q8_d, 0) hi_d + min(q8_d, 0) lo_d with q8 = rint(q / 2^a) and the
 // page's bounds hi, lo in units of 2^b.  The sum is a product of whole numbers over 2 D channels: v_mfma_i32_16x16x64_i8,
 // exact in any order.  A wave scores 16 pages for 16 columns: `width` columns (a power of two) a token, the group's heads.
-constexpr float kNotFinite = INFINITY;  // score of a page that holds what is not finite, or is not there: over all others, which end at the largest float
+// Score of a page that holds what is not finite, or is not there: over all others, which end at the largest float.
+constexpr float kNotFinite = INFINITY;
 template <int D>
 struct ScoreCols {  // this lane's column: channels k * 64 + q4 * 16 .. + 16 in 8 bits
     u4 pos[D / 64], neg[D / 64];
@@ -1798,8 +1799,9 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvCache c, KvBatch
     }
 }
 
-// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds; rows [row0, row1) of them.  One token of 1024 pages,
-// 8 heads: 7 us and 6 to 10, chains of loads; 32 tokens of up to 1563: 17 us, 2.8 TB/s of bounds, and 10.
+// The same in two kernels, scores by way of memory, where few tokens have many pages, or more than LDS holds; for rows [row0, row1),
+// as many as the scratch has room for.  One token of 1024 pages, 8 heads: 7 us and 6 to 10, chains of loads; 32 tokens of up to 1563:
+// 17 us, 2.8 TB/s of bounds, and 10.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_kv_score(KvCache c, KvBatch bt, AttendArgs a, uint32_t per, uint32_t chunks, uint32_t row0, uint32_t row1) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -640,9 +640,9 @@ gvdb_status gvdb_kv_attend_device(const gvdb_kv_cache* cache, const gvdb_kv_batc
  * an upper estimate of the page's largest q . k (2^a: the smallest under which
  * |q8| <= 127); the sum runs over whole numbers and is exact (scores over 2^128
  * are equal, and powers 2^a times the bounds' below 2^-126 are 2^-126).  A page
- * whose bounds are not finite, or that is not there, comes first.  chosen: device int32
- * [rows][kv_heads][top], ascending positions in the page table, -1 behind the
- * last, or NULL. */
+ * whose bounds are not finite, or that is not there, comes first.  chosen:
+ * device int32 [rows][kv_heads][top], ascending positions in the page table, -1
+ * behind the last, or NULL. */
 gvdb_status gvdb_kv_attend_topk_device(const gvdb_kv_cache* cache, const gvdb_kv_batch* batch, const gvdb_kv_rows* q,
                                        uint32_t q_heads, float scale, uint32_t top, uint32_t first, uint32_t recent,
                                        const gvdb_kv_rows* out, int32_t* chosen, float* lse, void* scratch,
