@@ -1456,8 +1456,10 @@ __global__ __launch_bounds__(256) void k_kv_combine(KvCache c, KvBatch bt, Atten
 // Score of a page for a query head: 2^(a + b) * sum_d max(q8_d, 0) hi_d + min(q8_d, 0) lo_d with q8 = rint(q / 2^a) and the
 // page's bounds hi, lo in units of 2^b.  The sum is a product of whole numbers over 2 D channels: v_mfma_i32_16x16x64_i8,
 // exact in any order.  A wave scores 16 pages for 16 columns: `width` columns (a power of two) a token, the group's heads.
+
 // Score of a page that holds what is not finite, or is not there: over all others, which end at the largest float.
 constexpr float kNotFinite = INFINITY;
+
 template <int D>
 struct ScoreCols {  // this lane's column: channels k * 64 + q4 * 16 .. + 16 in 8 bits
     u4 pos[D / 64], neg[D / 64];

@@ -457,3 +457,33 @@ def test_row_bounds_and_lengths_that_make_no_sense(kv):  # noqa: F811
             assert [bool(torch.isnan(x).all()) for x in out] == nan and bool((out[0] == 0).all())
         st.cache.append(q[:, :2], q[:, :2], st.table[:, :1].contiguous(), i32([2 ** 31 - 1, 33]))  # behind the table: skipped
         assert torch.equal(k, st.cache.pool)
+
+
+def test_two_threads_at_once(kv):  # noqa: F811
+    """Two callers of one cache, each on a stream of its own, with calls that need scratch: neither sees the other's."""
+    import threading
+
+    st = Store(kv, 140, "bf16", 2, 128, 64, (3000, 500))
+    shapes = [queries(141 + i, "bf16", (1, 1), 8, 128).cuda() for i in range(2)]
+    lens = st.lengths()
+    want = [(st.cache.attend(q, st.table, lens), *st.cache.attend_topk(q, st.table, lens, 6)) for q in shapes]
+    assert path(st.cache, shapes[0], st.table, lens) == LINE
+    torch.cuda.synchronize()
+    wrong, done = [], []
+
+    def caller(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(60):
+                got = (st.cache.attend(shapes[i], st.table, lens), *st.cache.attend_topk(shapes[i], st.table, lens, 6))
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+        torch.cuda.current_stream().synchronize()
+        done.append(i)
+
+    threads = [threading.Thread(target=caller, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert sorted(done) == [0, 1] and not wrong
